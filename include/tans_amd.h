@@ -320,6 +320,56 @@ int tans_fp8_gemm_fused_noalloc(const void* comp, int64_t comp_bytes, const int6
 int tans_fp8_gemm_raw(const void* w, int64_t R, int64_t C, const void* x, int64_t B,
                       float scale, void* y, void* stream);
 
+/* ---------------- A layer with FP8 weights (no counterpart in the
+ * reference) ------------------------------------------------------------
+ * Rows are row-major and contiguous; bf16 rows have a multiple of 16
+ * elements and 16-byte alignment, FP8 bytes are E4M3FN.                  */
+
+/* Root-mean-square norm with the residual's addition, output in 8 bits:
+ *   h = x + residual                    (fp32; stored as bf16, nearest even)
+ *   y = h * weight / sqrt(mean(h^2) + eps)            (fp32, from unrounded h)
+ *   scale[m] = max(max over the row of |y|, 2^-100) / 448
+ *   q = E4M3FN(y / scale[m]), nearest even
+ * A row that holds a NaN or an infinity gets NaN bytes in its place at
+ * least, and a scale that is not finite; other rows are not affected.
+ *   x, residual, h  bf16 [M, D]; residual NULL: h = x, not stored (h unused).
+ *                   h may be x or residual
+ *   weight          bf16 [D]
+ *   q               E4M3FN [M, D]; scale float [M]
+ * M >= 0, D a multiple of 16 in 16 .. 2^24.                              */
+int tans_fp8_rmsnorm(const void* x, const void* residual, const void* weight, int64_t M, int64_t D,
+                     float eps, void* q, float* scale, void* h, void* stream);
+
+/* Rows of bf16 x [M, D] to 8 bits: scale and q of tans_fp8_rmsnorm with
+ * y = x.                                                                 */
+int tans_fp8_quantize_rows(const void* x, int64_t M, int64_t D, void* q, float* scale,
+                           void* stream);
+
+/* Matrix product of FP8 rows with FP8 weights and its epilogue:
+ *   v[m][n] = (sum_k a[m][k] * w[n][k]) * a_scale[m] * (w_scale[n] * scale) + bias[n]
+ *   y[m][n] = act(v[m][n]) + residual[m][n]                      (N = R)
+ *   gated: y[m][j] = act(v[m][j]) * v[m][R / 2 + j] + residual[m][j]  (N = R / 2)
+ * fp32 accumulation in a fixed order, one rounding to bf16 (nearest even).
+ *   a          E4M3FN [M, C]; w E4M3FN [R, C]; C a multiple of 16, 16 .. 2^22
+ *   a_scale    float [M] or NULL (1); w_scale float [R] or NULL (1)
+ *   bias       bf16 [R] or NULL; residual bf16 [M, N] or NULL
+ *   activation TANS_ACT_*
+ *   y          bf16 [M, N]; may be residual
+ *   workspace  device scratch of tans_fp8_linear_workspace's size, 16-byte
+ *              aligned (contents on entry do not matter; NULL if 0)        */
+enum {
+    TANS_ACT_NONE = 0,
+    TANS_ACT_RELU = 1,
+    TANS_ACT_SILU = 2,
+    TANS_ACT_GELU = 3,        /* x * Phi(x)                               */
+    TANS_ACT_GELU_TANH = 4    /* its tanh form                            */
+};
+int tans_fp8_linear_workspace(int64_t M, int64_t R, int64_t C, int32_t gated, int64_t* bytes);
+int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const float* w_scale,
+                    float scale, const void* bias, const void* residual, int32_t activation,
+                    int32_t gated, int64_t M, int64_t R, int64_t C, void* workspace,
+                    int64_t workspace_bytes, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,5 @@
 """Build libtans_amd.so in-tree: the CPU codec (g++, OpenMP) and the gfx950
-HIP kernels and GPU encoder (hipcc), linked into one shared library next to the Python
+HIP kernels, GPU encoder and layer kernels (hipcc), linked into one shared library next to the Python
 package (rans_vectoradd/libtans_amd.so).
 
     python tans-vectoradd_amd/build.py [--asm]
@@ -33,6 +33,7 @@ HIP_FLAGS = [
 # compare and a second exec mask: 6 VALU and 6 SALU per tile), so it is off
 # for kernels.hip.
 KERNEL_FLAGS = ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
+LAYER_SOURCES = ["rows", "linear"]   # norm and rounding of rows; the FP8 product
 CXX_FLAGS = ["-O3", "-fPIC", "-std=c++17", "-fopenmp", "-Wall", "-Wextra"]
 
 
@@ -57,12 +58,15 @@ def build(asm: bool = False) -> str:
     _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "-c", os.path.join(CSRC, "kernels.hip"),
           "-o", kern_o])
     _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, "encode.hip"), "-o", enc_o])
+    layer_o = [os.path.join(BUILD, f"{name}.o") for name in LAYER_SOURCES]
+    for name, obj in zip(LAYER_SOURCES, layer_o):
+        _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj])
     if asm:
         _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "--cuda-device-only", "-S",
               os.path.join(CSRC, "kernels.hip"), "-o", os.path.join(BUILD, "kernels.s")])
     tmp = OUT + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, codec_o, kern_o, enc_o,
-          "-lgomp"])
+          *layer_o, "-lgomp"])
     os.replace(tmp, OUT)
     return OUT
 

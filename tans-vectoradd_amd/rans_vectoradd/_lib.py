@@ -38,6 +38,10 @@ EXPORTS = (
     "tans_gpu_encode_matrix_begin",
     "tans_gpu_encode_packed_begin",
     "tans_gpu_encode_packed_finish",
+    "tans_fp8_rmsnorm",
+    "tans_fp8_quantize_rows",
+    "tans_fp8_linear_workspace",
+    "tans_fp8_linear",
 )
 
 TANS_LANES = 64
@@ -92,6 +96,11 @@ for _name, _args in {
     "tans_gpu_encode_finish": [_I64, _I64, _I32, _P, _P, _P, _I64, _P],
     "tans_gpu_encode_packed_begin": [_P, _I64, _I64, _P, _P, _I32, _P, _I64, _P, _P, _P, _P],
     "tans_gpu_encode_packed_finish": [_I64, _I64, _I32, _P, _P, _P, _I64, _P],
+    "tans_fp8_rmsnorm": [_P, _P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P, _P],
+    "tans_fp8_quantize_rows": [_P, _I64, _I64, _P, _P, _P],
+    "tans_fp8_linear_workspace": [_I64, _I64, _I64, _I32, ctypes.POINTER(_I64)],
+    "tans_fp8_linear": [_P, _P, _P, _P, ctypes.c_float, _P, _P, _I32, _I32, _I64, _I64, _I64, _P,
+                        _I64, _P, _P],
 }.items():
     getattr(lib, _name).restype = ctypes.c_int
     getattr(lib, _name).argtypes = _args
