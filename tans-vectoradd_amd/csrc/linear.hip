@@ -7,6 +7,12 @@
 //
 // a and w hold E4M3FN bytes; the products of v_mfma_f32_16x16x128_f8f6f4 are
 // exact and summed in 32 bits; y is rounded once, to bf16.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "launch.h"
 #include "layer.h"
 
 namespace {
@@ -15,6 +21,8 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 
 constexpr int64_t kMaxCols = int64_t(1) << 22;   // a tile's rows stay below 2^32 bytes
 
+constexpr float kLog2e = 1.44269504f;
+
 struct Epilogue {
     const float* a_scale;        // [M] or null (1)
     const float* w_scale;        // [R] or null (1)
@@ -22,17 +30,36 @@ struct Epilogue {
     const uint16_t* residual;    // bf16 [M, N] or null
     uint16_t* y;                 // bf16 [M, N]
     float scale;
-    int act;
+    float lo;                    // kClip: the least value
+    float c1, c3;                // kSigmoid: of the sigmoid's argument, times log2 e
 };
 
-__device__ __forceinline__ float activate(float v, int act) {
-    switch (act) {
-        case TANS_ACT_RELU: return v < 0.0f ? 0.0f : v;   // a NaN stays one
-        case TANS_ACT_SILU: return v / (1.0f + expf(-v));
-        case TANS_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-        case TANS_ACT_GELU_TANH:
-            return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
-        default: return v;
+// The activations in three forms, each a kernel of its own:
+//   kClip     max(v, lo): none (lo = -infinity) and ReLU (a NaN stays one)
+//   kSigmoid  v * sigmoid(b1 v + b3 v^3): SiLU (b1 = 1, b3 = 0) and GELU's tanh
+//             form, (1 + tanh(u)) / 2 = sigmoid(2 u)
+//   kErf      v Phi(v), erfc by Abramowitz and Stegun 7.1.26 (absolute error
+//             below 1.5e-7)
+enum Act { kClip, kSigmoid, kErf };
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v, const Epilogue& e) {
+    if constexpr (ACT == kClip) {
+        return v < e.lo ? e.lo : v;
+    } else if constexpr (ACT == kSigmoid) {
+        // the square is kept finite, for b3 = 0 times it
+        const float sq = __builtin_fminf(v * v, 1e30f);
+        const float x = v * __builtin_fmaf(e.c3, sq, e.c1);
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x));
+    } else {
+        const float x = __builtin_fabsf(v) * 0.70710678f;
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+        float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+        p = __builtin_fmaf(p, t, 1.421413741f);
+        p = __builtin_fmaf(p, t, -0.284496736f);
+        p = __builtin_fmaf(p, t, 0.254829592f) * t;
+        const float half_erfc = 0.5f * p * __builtin_amdgcn_exp2f(-1.44269504f * x * x);
+        return v * (v < 0.0f ? half_erfc : 1.0f - half_erfc);
     }
 }
 
@@ -41,7 +68,7 @@ __device__ __forceinline__ float activate(float v, int act) {
 // registers: lane l holds row l % 16 of either and, of each 128 columns,
 // columns 32 (l / 16) .. + 31.  Of the 16 x 16 products, lane l gets those of
 // a's row l % 16 with weight rows 4 (l / 16) .. + 3.
-template <bool GATED>
+template <bool GATED, int ACT>
 __global__ __launch_bounds__(256) void linear_kernel(const uint8_t* __restrict__ a,
                                                      const uint8_t* __restrict__ w, int64_t M,
                                                      int64_t N, int64_t C, Epilogue e) {
@@ -78,11 +105,341 @@ __global__ __launch_bounds__(256) void linear_kernel(const uint8_t* __restrict__
             v = v * sa * ((e.w_scale ? e.w_scale[col] : 1.0f) * e.scale);
             return e.bias ? v + bf16_lo(e.bias[col]) : v;
         };
-        float v = activate(scaled(acc[i], c), e.act);
+        float v = activate<ACT>(scaled(acc[i], c), e);
         if (GATED) v *= scaled(up[i], N + c);
         if (e.residual) v += bf16_lo(e.residual[m * N + c]);
         e.y[m * N + c] = (uint16_t)bf16_pack(v, 0.0f);
     }
+}
+
+
+// Scale and bias of w's rows first + c .. first + c + CN - 1, of which those
+// with c + i < N exist (the others are repeats of the last).
+template <int CN>
+__device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_t c, int64_t N,
+                                        float (&ws)[CN], float (&bs)[CN]) {
+    #pragma unroll
+    for (int i = 0; i < CN; i++) {
+        ws[i] = 1.0f;
+        bs[i] = 0.0f;
+    }
+    uint16_t b[CN];
+    if (c + CN <= N) {
+        if (e.w_scale) __builtin_memcpy(ws, e.w_scale + first + c, sizeof(ws));
+        if (e.bias) __builtin_memcpy(b, e.bias + first + c, sizeof(b));
+    } else {
+        #pragma unroll
+        for (int i = 0; i < CN; i++) {
+            const int64_t n = first + (c + i < N ? c + i : N - 1);
+            if (e.w_scale) ws[i] = e.w_scale[n];
+            if (e.bias) b[i] = e.bias[n];
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < CN; i++) {
+        ws[i] *= e.scale;
+        if (e.bias) bs[i] = bf16_lo(b[i]);
+    }
+}
+
+// ---------------------------------------------------------------------
+// Tiles of 256 rows of a by 256 rows of w, for products with many rows.
+// ---------------------------------------------------------------------
+constexpr int kTile = 256;          // rows of either operand
+constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
+constexpr int kStep = 128;          // columns (bytes) of a step
+constexpr int kTileBytes = kTile * kStep;
+constexpr int kTileWaves = 4;
+// An offset past every tile's bytes (kTile * kMaxCols = 2^30), also with a
+// tile's row offset added
+constexpr uint32_t kOut = 0x80000000u;
+
+// 16 bytes a lane from memory to LDS, lane l's to lds + 16 l; zeros from
+// offsets out of range.
+__device__ __forceinline__ void load_lds(const Rsrc& src, uint8_t* lds, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16,
+                                             (int)offset, 0, 0, 0);
+}
+
+// x, of which the compiler knows nothing any more
+__device__ __forceinline__ uint32_t opaque_s(uint32_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t opaque_v(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
+    return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
+               (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+__device__ __forceinline__ v4f mfma(const v8i& w, const v8i& a, const v4f& c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
+}
+
+// Where a workgroup's tiles lie: the tile sequence takes groups of kGroupM
+// tiles of a's rows, in each of them w's tiles in order and the group's row
+// tiles innermost; an eighth of the sequence goes to each of the 8 XCDs
+// (workgroup b runs on XCD b % 8), so that the tiles an XCD works on at a time
+// share their rows of a and w in its L2.
+constexpr int kXcds = 8;
+constexpr int kGroupM = 8;
+
+struct TileMap {
+    int tiles_m, tiles_n;
+    __device__ __forceinline__ int count() const { return tiles_m * tiles_n; }
+    // the i-th tile of workgroup b of `blocks`, or -1
+    __device__ __forceinline__ int at(int i, int b, int blocks) const {
+        const int xcd = b % kXcds, T = count();
+        const int per = T / kXcds, more = T % kXcds;
+        const int first = xcd * per + (xcd < more ? xcd : more);
+        const int n = per + (xcd < more ? 1 : 0);
+        const int peers = (blocks - xcd + kXcds - 1) / kXcds;
+        const int k = i * peers + b / kXcds;
+        return k < n ? first + k : -1;
+    }
+    __device__ __forceinline__ void place(int t, int& tm, int& tn) const {
+        const int group = t / (kGroupM * tiles_n);
+        const int m_first = group * kGroupM;
+        const int gm = tiles_m - m_first < kGroupM ? tiles_m - m_first : kGroupM;
+        const int in = t - group * kGroupM * tiles_n;
+        tm = m_first + in % gm;
+        tn = in / gm;
+    }
+};
+
+template <bool GATED, int ACT>
+__global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
+    const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
+    TileMap map, Epilogue e) {
+    __shared__ __attribute__((aligned(1024))) uint8_t sa0[kTileBytes], sa1[kTileBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sw0[kTileBytes], sw1[kTileBytes];
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int r = lane & 15, g = lane >> 4;
+    const uint32_t row_bytes = (uint32_t)C;
+    const int steps = (int)((C + 2 * kStep - 1) / (2 * kStep)) * 2;   // even
+
+    // Loads: one instruction brings 8 rows of 128 bytes, lane l the 16 bytes
+    // that belong at position l % 8 of row l / 8.  A row's 16-byte pieces are
+    // permuted by an exclusive or with a key of the row, see `frag`.
+    const int lrow = wave * 8 + (lane >> 3), lpos = lane & 7;
+    const int akey = ((lane >> 4) & 3) | ((wave & 1) << 2);
+    const int wkey = ((lane >> 4) & 1) | ((wave >> 1) << 1);      // and 4 for odd instructions
+    const uint32_t acol = (uint32_t)(lpos ^ akey) * 16, wcol = (uint32_t)(lpos ^ wkey) * 16;
+    const uint32_t lbase = (uint32_t)lrow * row_bytes;
+
+    struct Src { Rsrc a, w0, w1; int64_t m0, n0; } cur, nxt;
+    auto source = [&](int t) {
+        Src s;
+        if (t < 0) {   // nothing: every load is out of range
+            s.a = s.w0 = s.w1 = rsrc(a, 0);
+            s.m0 = s.n0 = 0;
+            return s;
+        }
+        int tm, tn;
+        map.place(t, tm, tn);
+        s.m0 = (int64_t)tm * kTile;
+        s.n0 = (int64_t)tn * (GATED ? kHalf : kTile);
+        auto rows = [&](int64_t have, int most) {
+            return (uint32_t)(have < 0 ? 0 : have < most ? have : most) * row_bytes;
+        };
+        s.a = rsrc(a + s.m0 * C, rows(M - s.m0, kTile));
+        s.w0 = rsrc(w + s.n0 * C, rows(N - s.n0, kHalf));
+        const int64_t second = GATED ? N + s.n0 : s.n0 + kHalf;
+        const uint32_t bytes1 = rows(GATED ? N - s.n0 : N - second, kHalf);
+        s.w1 = rsrc(bytes1 ? w + second * C : w, bytes1);
+        return s;
+    };
+    // step k of a tile into a buffer; columns past C come as zeros
+    auto fetch = [&](const Src& s, int k, uint8_t* sa, uint8_t* sw) {
+        const uint32_t k0 = (uint32_t)k * kStep;
+        const uint32_t ao = k0 + acol < row_bytes ? lbase + k0 + acol : kOut;
+        const uint32_t wo[2] = {k0 + wcol < row_bytes ? lbase + k0 + wcol : kOut,
+                                k0 + (wcol ^ 64) < row_bytes ? lbase + k0 + (wcol ^ 64) : kOut};
+        // (opaque: otherwise all 64 LDS addresses are kept in registers)
+        uint32_t lds = wave * 1024;
+        lds = opaque_s(lds);
+        #pragma unroll
+        for (int j = 0; j < 8; j++)
+            load_lds(s.a, sa + lds + j * 4096, ao + (uint32_t)j * 32 * row_bytes);
+        #pragma unroll
+        for (int j = 0; j < 8; j++)
+            load_lds(j < 4 ? s.w0 : s.w1, sw + lds + j * 4096,
+                     wo[j & 1] + (uint32_t)(j & 3) * 32 * row_bytes);
+    };
+
+    // Fragments: lane (g, r) takes pieces g and 4 + g of its row.
+    const int key = r >> 1;
+    const uint32_t piece = (uint32_t)(((g ^ key) & 3) | (key & 4)) * 16;
+    uint32_t abase[2], wbase[2];
+    abase[0] = wm * 16384 + r * 128 + piece;
+    wbase[0] = wn * 8192 + (r >> 2) * 2048 + (r & 3) * 128 + piece;
+    abase[1] = abase[0] ^ 64;
+    wbase[1] = wbase[0] ^ 64;
+    // (opaque: otherwise the exclusive or is done, and kept, for every piece)
+    abase[1] = opaque_v(abase[1]);
+    wbase[1] = opaque_v(wbase[1]);
+    v8i fa[8], fw[8];     // 16 rows each; fw[4 h + f]: half h
+    v4f acc[8][8];
+    auto zero = [&]() {
+        #pragma unroll
+        for (int i = 0; i < 8; i++)
+            #pragma unroll
+            for (int j = 0; j < 8; j++) acc[i][j] = v4f{0, 0, 0, 0};
+    };
+    auto frag = [&](const uint8_t* p, const uint32_t (&o)[2]) {
+        return join(*reinterpret_cast<const v4u*>(p + o[0]), *reinterpret_cast<const v4u*>(p + o[1]));
+    };
+    auto read_a = [&](auto H, const uint8_t* sa) {
+        constexpr int h = decltype(H)::value;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) fa[4 * h + i] = frag(sa + (4 * h + i) * 2048, abase);
+    };
+    auto read_w = [&](auto H, const uint8_t* sw) {
+        constexpr int h = decltype(H)::value;
+        #pragma unroll
+        for (int f = 0; f < 4; f++) fw[4 * h + f] = frag(sw + h * 16384 + f * 512, wbase);
+    };
+    auto multiply = [&](auto HA, auto HW) {
+        constexpr int ha = decltype(HA)::value, hw = decltype(HW)::value;
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            #pragma unroll
+            for (int f = 0; f < 4; f++)
+                acc[4 * ha + i][4 * hw + f] = mfma(fw[4 * hw + f], fa[4 * ha + i], acc[4 * ha + i][4 * hw + f]);
+    };
+    constexpr std::integral_constant<int, 0> I0{};
+    constexpr std::integral_constant<int, 1> I1{};
+    // A barrier for which every wave's loads into LDS have arrived (the
+    // compiler's own waits cover a wave's own reads only).
+    auto arrive = []() {
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+        __syncthreads();
+    };
+    // 8 LDS reads spread over 16 products
+    auto spread = [&]() {
+        #pragma unroll
+        for (int i = 0; i < 8; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Step on the buffer (sa, sw), a's half 0 and w's half X in registers; the
+    // other buffer (na, nw) holds the next step from the middle on, and (sa, sw)
+    // is filled with step k2 of s2.  Leaves a's half 0 and w's half Y of the
+    // next step in registers.
+    auto step = [&](auto X, auto Y, uint8_t* sa, uint8_t* sw, uint8_t* na, uint8_t* nw,
+                    const Src& s2, int k2) {
+        read_w(Y, sw);
+        multiply(I0, X);
+        spread();
+        read_a(I1, sa);
+        multiply(I0, Y);
+        spread();
+        arrive();            // the next step has come; nobody reads (sa, sw) any more
+        fetch(s2, k2, sa, sw);
+        __builtin_amdgcn_sched_barrier(0);
+        read_a(I0, na);
+        multiply(I1, Y);
+        spread();
+        read_w(Y, nw);
+        multiply(I1, X);
+        spread();
+    };
+
+    int i = 0;
+    int t = map.at(0, blockIdx.x, gridDim.x);
+    if (t < 0) return;
+    cur = source(t);
+    fetch(cur, 0, sa0, sw0);
+    arrive();
+    fetch(cur, 1, sa1, sw1);
+    while (true) {
+        const int t_next = map.at(++i, blockIdx.x, gridDim.x);
+        nxt = source(t_next);
+        // (the last step of a tile before has read these pieces too, but not
+        // kept them over the epilogue)
+        read_a(I0, sa0);
+        read_w(I0, sw0);
+        zero();
+        for (int k = 2; k <= steps; k += 2) {
+            // the last two steps fetch the next tile's first two
+            const Src& s2 = k == steps ? nxt : cur;
+            const int k2 = k == steps ? 0 : k;
+            step(I0, I1, sa0, sw0, sa1, sw1, s2, k2);
+            step(I1, I0, sa1, sw1, sa0, sw0, s2, k2 + 1);
+        }
+
+        // lane (g, r): row r of each of 8 groups of 16 rows of a, and of each
+        // half of w's rows 16 consecutive ones from 64 wn + 16 g on
+        float ws[2][16], bs[2][16];
+        int64_t col[2];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            col[h] = cur.n0 + (GATED ? 0 : h * kHalf) + wn * 64 + g * 16;
+            columns(e, (GATED && h ? N : 0), col[h], N, ws[h], bs[h]);
+        }
+        const bool vec = N % 8 == 0;
+        #pragma unroll
+        for (int im = 0; im < 8; im++) {
+            const int64_t m = cur.m0 + wm * 128 + im * 16 + r;
+            if (m >= M) break;
+            const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
+            #pragma unroll
+            for (int h = 0; h < (GATED ? 1 : 2); h++) {
+                float v[16];
+                #pragma unroll
+                for (int c = 0; c < 16; c++) {
+                    v[c] = acc[im][4 * h + c / 4][c % 4] * sm * ws[h][c] + bs[h][c];
+                    v[c] = activate<ACT>(v[c], e);
+                    if (GATED) v[c] *= acc[im][4 + c / 4][c % 4] * sm * ws[1][c] + bs[1][c];
+                }
+                const int64_t o = m * N + col[h];
+                if (vec && col[h] + 16 <= N) {
+                    #pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        if (e.residual) {
+                            const v4u u = *reinterpret_cast<const v4u*>(e.residual + o + 8 * b);
+                            #pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                v[8 * b + 2 * c] += bf16_lo(u[c]);
+                                v[8 * b + 2 * c + 1] += bf16_hi(u[c]);
+                            }
+                        }
+                        v4u u;
+                        #pragma unroll
+                        for (int c = 0; c < 4; c++) u[c] = bf16_pack(v[8 * b + 2 * c], v[8 * b + 2 * c + 1]);
+                        *reinterpret_cast<v4u*>(e.y + o + 8 * b) = u;
+                    }
+                } else {
+                    for (int c = 0; c < 16 && col[h] + c < N; c++) {
+                        if (e.residual) v[c] += bf16_lo(e.residual[o + c]);
+                        e.y[o + c] = (uint16_t)bf16_pack(v[c], 0.0f);
+                    }
+                }
+            }
+        }
+        if (t_next < 0) break;
+        t = t_next;
+        cur = nxt;
+    }
+}
+
+// f(gated, activation form) with both as types
+template <class F>
+void for_kind(bool gated, int act, F&& f) {
+    auto with = [&](auto G) {
+        if (act == kErf) f(G, std::integral_constant<int, kErf>{});
+        else if (act == kSigmoid) f(G, std::integral_constant<int, kSigmoid>{});
+        else f(G, std::integral_constant<int, kClip>{});
+    };
+    if (gated) with(std::true_type{}); else with(std::false_type{});
 }
 
 }  // namespace
@@ -116,16 +473,37 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
     if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return fail(TANS_EINVAL, "linear: workspace too small, null or misaligned (16 bytes)");
     const int64_t N = gated ? R / 2 : R;
+    const float tanh_c1 = 2.0f * 0.79788456f * kLog2e;   // 2 sqrt(2 / pi)
+    const bool tanh_form = activation == TANS_ACT_GELU_TANH;
+    const Epilogue e = {a_scale, w_scale, (const uint16_t*)bias, (const uint16_t*)residual,
+                        (uint16_t*)y, scale,
+                        activation == TANS_ACT_RELU ? 0.0f : -INFINITY,
+                        tanh_form ? tanh_c1 : kLog2e, tanh_form ? 0.044715f * tanh_c1 : 0.0f};
+    const int act = activation == TANS_ACT_GELU ? kErf
+                    : activation == TANS_ACT_SILU || tanh_form ? kSigmoid : kClip;
+    if (M > 128) {
+        const TileMap map = {(int)((M + kTile - 1) / kTile), (int)((N + (gated ? kHalf : kTile) - 1) / (gated ? kHalf : kTile))};
+        const int64_t tiles = (int64_t)map.tiles_m * map.tiles_n;
+        const int cus = tans_internal_cu_count();
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, cus)), dim3(256), 0,
+                               (hipStream_t)stream, (const uint8_t*)a, (const uint8_t*)w, M, N, C, map, e);
+        };
+        for_kind(gated, act, [&](auto G, auto A) {
+            launch(linear_tile_kernel<decltype(G)::value, decltype(A)::value>);
+        });
+        return hip_check(hipGetLastError(), "linear_tile_kernel launch");
+    }
     const int64_t blocks = (N + 63) / 64 * ((M + 15) / 16);
     if (blocks > UINT32_MAX / 256) return fail(TANS_EINVAL, "linear: too many outputs for one call");
     const dim3 grid((unsigned)blocks);
-    const Epilogue e = {a_scale, w_scale, (const uint16_t*)bias, (const uint16_t*)residual,
-                        (uint16_t*)y, scale, activation};
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const uint8_t*)a,
                            (const uint8_t*)w, M, N, C, e);
     };
-    if (gated) launch(linear_kernel<true>); else launch(linear_kernel<false>);
+    for_kind(gated, act, [&](auto G, auto A) {
+        launch(linear_kernel<decltype(G)::value, decltype(A)::value>);
+    });
     return hip_check(hipGetLastError(), "linear_kernel launch");
 }
 
