@@ -255,22 +255,28 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         s.w1 = rsrc(bytes1 ? w + second * C : w, bytes1);
         return s;
     };
-    // step k of a tile into a buffer; columns past C come as zeros
-    auto fetch = [&](const Src& s, int k, uint8_t* sa, uint8_t* sw) {
+    // Step k of a tile into a buffer, in 16 loads; columns past C come as zeros.
+    struct Fetch { uint32_t a, w[2], lds; } at;
+    auto aim = [&](int k) {
         const uint32_t k0 = (uint32_t)k * kStep;
-        const uint32_t ao = k0 + acol < row_bytes ? lbase + k0 + acol : kOut;
-        const uint32_t wo[2] = {k0 + wcol < row_bytes ? lbase + k0 + wcol : kOut,
-                                k0 + (wcol ^ 64) < row_bytes ? lbase + k0 + (wcol ^ 64) : kOut};
-        // (opaque: otherwise all 64 LDS addresses are kept in registers)
-        uint32_t lds = wave * 1024;
-        lds = opaque_s(lds);
+        at.a = k0 + acol < row_bytes ? lbase + k0 + acol : kOut;
+        at.w[0] = k0 + wcol < row_bytes ? lbase + k0 + wcol : kOut;
+        at.w[1] = k0 + (wcol ^ 64) < row_bytes ? lbase + k0 + (wcol ^ 64) : kOut;
+        at.lds = opaque_s(wave * 1024);   // (otherwise all 64 LDS addresses stay in registers)
+    };
+    auto fetch_a = [&](const Src& s, uint8_t* sa, int j) {
+        load_lds(s.a, sa + at.lds + j * 4096, at.a + (uint32_t)j * 32 * row_bytes);
+    };
+    auto fetch_w = [&](const Src& s, uint8_t* sw, int j) {
+        load_lds(j < 4 ? s.w0 : s.w1, sw + at.lds + j * 4096,
+                 at.w[j & 1] + (uint32_t)(j & 3) * 32 * row_bytes);
+    };
+    auto fetch = [&](const Src& s, int k, uint8_t* sa, uint8_t* sw) {
+        aim(k);
         #pragma unroll
-        for (int j = 0; j < 8; j++)
-            load_lds(s.a, sa + lds + j * 4096, ao + (uint32_t)j * 32 * row_bytes);
+        for (int j = 0; j < 8; j++) fetch_a(s, sa, j);
         #pragma unroll
-        for (int j = 0; j < 8; j++)
-            load_lds(j < 4 ? s.w0 : s.w1, sw + lds + j * 4096,
-                     wo[j & 1] + (uint32_t)(j & 3) * 32 * row_bytes);
+        for (int j = 0; j < 8; j++) fetch_w(s, sw, j);
     };
 
     // Fragments: lane (g, r) takes pieces g and 4 + g of its row.
@@ -292,26 +298,31 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
             #pragma unroll
             for (int j = 0; j < 8; j++) acc[i][j] = v4f{0, 0, 0, 0};
     };
-    auto frag = [&](const uint8_t* p, const uint32_t (&o)[2]) {
-        return join(*reinterpret_cast<const v4u*>(p + o[0]), *reinterpret_cast<const v4u*>(p + o[1]));
-    };
-    auto read_a = [&](auto H, const uint8_t* sa) {
-        constexpr int h = decltype(H)::value;
+    // half s % 2 of fragment s / 2 of a half, s = 0 .. 7
+    auto set = [](v8i& f, int half, const v4u& u) {
         #pragma unroll
-        for (int i = 0; i < 4; i++) fa[4 * h + i] = frag(sa + (4 * h + i) * 2048, abase);
+        for (int i = 0; i < 4; i++) f[4 * half + i] = (int)u[i];
     };
-    auto read_w = [&](auto H, const uint8_t* sw) {
-        constexpr int h = decltype(H)::value;
-        #pragma unroll
-        for (int f = 0; f < 4; f++) fw[4 * h + f] = frag(sw + h * 16384 + f * 512, wbase);
+    auto read_a = [&](int h, const uint8_t* sa, int s) {
+        set(fa[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(sa + (4 * h + s / 2) * 2048 + abase[s % 2]));
     };
-    auto multiply = [&](auto HA, auto HW) {
+    auto read_w = [&](int h, const uint8_t* sw, int s) {
+        set(fw[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(sw + h * 16384 + s / 2 * 512 + wbase[s % 2]));
+    };
+    // The 16 products of halves HA and HW in 8 slots of two, each with what
+    // `with` issues for it (LDS reads for the next phase, loads).
+    auto multiply = [&](auto HA, auto HW, auto&& with) {
         constexpr int ha = decltype(HA)::value, hw = decltype(HW)::value;
         #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int s = 0; s < 8; s++) {
+            with(s);
             #pragma unroll
-            for (int f = 0; f < 4; f++)
-                acc[4 * ha + i][4 * hw + f] = mfma(fw[4 * hw + f], fa[4 * ha + i], acc[4 * ha + i][4 * hw + f]);
+            for (int p = 2 * s; p < 2 * s + 2; p++) {
+                v4f& c = acc[4 * ha + p / 4][4 * hw + p % 4];
+                c = mfma(fw[4 * hw + p % 4], fa[4 * ha + p / 4], c);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     constexpr std::integral_constant<int, 0> I0{};
     constexpr std::integral_constant<int, 1> I1{};
@@ -321,36 +332,25 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
         __syncthreads();
     };
-    // 8 LDS reads spread over 16 products
-    auto spread = [&]() {
-        #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
     // Step on the buffer (sa, sw), a's half 0 and w's half X in registers; the
     // other buffer (na, nw) holds the next step from the middle on, and (sa, sw)
     // is filled with step k2 of s2.  Leaves a's half 0 and w's half Y of the
     // next step in registers.
     auto step = [&](auto X, auto Y, uint8_t* sa, uint8_t* sw, uint8_t* na, uint8_t* nw,
                     const Src& s2, int k2) {
-        read_w(Y, sw);
-        multiply(I0, X);
-        spread();
-        read_a(I1, sa);
-        multiply(I0, Y);
-        spread();
+        constexpr int y = decltype(Y)::value;
+        multiply(I0, X, [&](int s) { read_w(y, sw, s); });
+        multiply(I0, Y, [&](int s) { read_a(1, sa, s); });
         arrive();            // the next step has come; nobody reads (sa, sw) any more
-        fetch(s2, k2, sa, sw);
-        __builtin_amdgcn_sched_barrier(0);
-        read_a(I0, na);
-        multiply(I1, Y);
-        spread();
-        read_w(Y, nw);
-        multiply(I1, X);
-        spread();
+        aim(k2);
+        multiply(I1, Y, [&](int s) {
+            read_a(0, na, s);
+            fetch_a(s2, sa, s);
+        });
+        multiply(I1, X, [&](int s) {
+            read_w(y, nw, s);
+            fetch_w(s2, sw, s);
+        });
     };
 
     int i = 0;
@@ -365,8 +365,11 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         nxt = source(t_next);
         // (the last step of a tile before has read these pieces too, but not
         // kept them over the epilogue)
-        read_a(I0, sa0);
-        read_w(I0, sw0);
+        #pragma unroll
+        for (int s = 0; s < 8; s++) {
+            read_a(0, sa0, s);
+            read_w(0, sw0, s);
+        }
         zero();
         for (int k = 2; k <= steps; k += 2) {
             // the last two steps fetch the next tile's first two
