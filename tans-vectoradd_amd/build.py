@@ -37,7 +37,8 @@ KERNEL_FLAGS = ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
 # AGPRs: selecting its matrix instructions with VGPR operands first and moving
 # them to AGPRs after register allocation leaves 29 copies in a loop of 128
 # matrix instructions instead of 336.
-LAYER_SOURCES = {"rows": [], "linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+LAYER_SOURCES = {"rows": [], "linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1",
+                            "-mllvm", "-disable-machine-licm=1"]}
 CXX_FLAGS = ["-O3", "-fPIC", "-std=c++17", "-fopenmp", "-Wall", "-Wextra"]
 
 

@@ -148,7 +148,7 @@ __device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_
 constexpr int kTile = 256;          // rows of either operand
 constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
 constexpr int kStep = 128;          // columns (bytes) of a step
-constexpr int kTileBytes = kTile * kStep;
+constexpr int kUnit = kHalf * kStep;
 constexpr int kTileWaves = 4;
 // An offset past every tile's bytes (kTile * kMaxCols = 2^30), also with a
 // tile's row offset added
@@ -215,8 +215,11 @@ template <bool GATED, int ACT>
 __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
     TileMap map, Epilogue e) {
-    __shared__ __attribute__((aligned(1024))) uint8_t sa0[kTileBytes], sa1[kTileBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t sw0[kTileBytes], sw1[kTileBytes];
+    // Two steps' operands, each in units of its own (128 rows, 16 KiB; the
+    // compiler tells loads into different arrays apart, and waits for none
+    // that a read does not need): s<operand><half><step % 2>
+    __shared__ __attribute__((aligned(1024))) uint8_t sa00[kUnit], sa10[kUnit], sw00[kUnit], sw10[kUnit];
+    __shared__ __attribute__((aligned(1024))) uint8_t sa01[kUnit], sa11[kUnit], sw01[kUnit], sw11[kUnit];
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int wm = wave >> 1, wn = wave & 1;
@@ -255,35 +258,26 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         s.w1 = rsrc(bytes1 ? w + second * C : w, bytes1);
         return s;
     };
-    // Step k of a tile into a buffer, in 16 loads; columns past C come as zeros.
-    struct Fetch { uint32_t a, w[2], lds; } at;
-    auto aim = [&](int k) {
-        const uint32_t k0 = (uint32_t)k * kStep;
-        at.a = k0 + acol < row_bytes ? lbase + k0 + acol : kOut;
-        at.w[0] = k0 + wcol < row_bytes ? lbase + k0 + wcol : kOut;
-        at.w[1] = k0 + (wcol ^ 64) < row_bytes ? lbase + k0 + (wcol ^ 64) : kOut;
-        at.lds = opaque_s(wave * 1024);   // (otherwise all 64 LDS addresses stay in registers)
+    // Half h of a's or w's rows of step k into a unit, in 4 loads (j) of each
+    // wave; columns past C come as zeros.  a's half h is rows 64 h .. of each
+    // 128, w's half h rows 128 h ...
+    auto fetch_a = [&](const Src& s, int k, int h, uint8_t* unit, int j) {
+        const uint32_t c = (uint32_t)k * kStep + acol;
+        load_lds(s.a, unit + opaque_s(wave * 1024) + j * 4096,
+                 (c < row_bytes ? lbase + c : kOut) +
+                     (uint32_t)((j >> 1) * 128 + h * 64 + (j & 1) * 32) * row_bytes);
     };
-    auto fetch_a = [&](const Src& s, uint8_t* sa, int j) {
-        load_lds(s.a, sa + at.lds + j * 4096, at.a + (uint32_t)j * 32 * row_bytes);
-    };
-    auto fetch_w = [&](const Src& s, uint8_t* sw, int j) {
-        load_lds(j < 4 ? s.w0 : s.w1, sw + at.lds + j * 4096,
-                 at.w[j & 1] + (uint32_t)(j & 3) * 32 * row_bytes);
-    };
-    auto fetch = [&](const Src& s, int k, uint8_t* sa, uint8_t* sw) {
-        aim(k);
-        #pragma unroll
-        for (int j = 0; j < 8; j++) fetch_a(s, sa, j);
-        #pragma unroll
-        for (int j = 0; j < 8; j++) fetch_w(s, sw, j);
+    auto fetch_w = [&](const Src& s, int k, int h, uint8_t* unit, int j) {
+        const uint32_t c = (uint32_t)k * kStep + (j & 1 ? wcol ^ 64 : wcol);
+        load_lds(h ? s.w1 : s.w0, unit + opaque_s(wave * 1024) + j * 4096,
+                 (c < row_bytes ? lbase + c : kOut) + (uint32_t)j * 32 * row_bytes);
     };
 
     // Fragments: lane (g, r) takes pieces g and 4 + g of its row.
     const int key = r >> 1;
     const uint32_t piece = (uint32_t)(((g ^ key) & 3) | (key & 4)) * 16;
     uint32_t abase[2], wbase[2];
-    abase[0] = wm * 16384 + r * 128 + piece;
+    abase[0] = wm * 8192 + r * 128 + piece;
     wbase[0] = wn * 8192 + (r >> 2) * 2048 + (r & 3) * 128 + piece;
     abase[1] = abase[0] ^ 64;
     wbase[1] = wbase[0] ^ 64;
@@ -303,11 +297,11 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         #pragma unroll
         for (int i = 0; i < 4; i++) f[4 * half + i] = (int)u[i];
     };
-    auto read_a = [&](int h, const uint8_t* sa, int s) {
-        set(fa[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(sa + (4 * h + s / 2) * 2048 + abase[s % 2]));
+    auto read_a = [&](int h, const uint8_t* unit, int s) {
+        set(fa[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 2 * 2048 + abase[s % 2]));
     };
-    auto read_w = [&](int h, const uint8_t* sw, int s) {
-        set(fw[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(sw + h * 16384 + s / 2 * 512 + wbase[s % 2]));
+    auto read_w = [&](int h, const uint8_t* unit, int s) {
+        set(fw[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 2 * 512 + wbase[s % 2]));
     };
     // The 16 products of halves HA and HW in 8 slots of two, each with what
     // `with` issues for it (LDS reads for the next phase, loads).
@@ -326,30 +320,46 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     };
     constexpr std::integral_constant<int, 0> I0{};
     constexpr std::integral_constant<int, 1> I1{};
-    // A barrier for which every wave's loads into LDS have arrived (the
-    // compiler's own waits cover a wave's own reads only).
-    auto arrive = []() {
-        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
-        __syncthreads();
+    // A barrier for which all but each wave's last LEFT loads into LDS have
+    // arrived, and its LDS reads (the compiler's own waits cover a wave's own
+    // loads only; __syncthreads would wait for all of them).
+    auto arrive = [](auto LEFT) {
+        constexpr int n = decltype(LEFT)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 0x070);   // vmcnt(n), lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     };
-    // Step on the buffer (sa, sw), a's half 0 and w's half X in registers; the
-    // other buffer (na, nw) holds the next step from the middle on, and (sa, sw)
-    // is filled with step k2 of s2.  Leaves a's half 0 and w's half Y of the
-    // next step in registers.
-    auto step = [&](auto X, auto Y, uint8_t* sa, uint8_t* sw, uint8_t* na, uint8_t* nw,
-                    const Src& s2, int k2) {
-        constexpr int y = decltype(Y)::value;
-        multiply(I0, X, [&](int s) { read_w(y, sw, s); });
-        multiply(I0, Y, [&](int s) { read_a(1, sa, s); });
-        arrive();            // the next step has come; nobody reads (sa, sw) any more
-        aim(k2);
+    constexpr std::integral_constant<int, 16> LEFT2{};   // the loads of two half steps
+    constexpr std::integral_constant<int, 24> LEFT3{};
+    // A step in two halves, on its units a0, a1, x, y (w's halves X and Y) and
+    // the next step's a0n, yn; a's half 0 and w's half X are in registers.  Each
+    // half reads two units and refills the two that the half before has read
+    // with the step after the next (k2 of s2), so that a load has two to three
+    // half steps to arrive in.  Leaves a's half 0 and w's half Y of the next step
+    // in registers.
+    auto step = [&](auto X, auto Y, uint8_t* a0, uint8_t* a1, uint8_t* x, uint8_t* y, uint8_t* a0n,
+                    uint8_t* yn, const Src& s2, int k2) {
+        constexpr int hx = decltype(X)::value, hy = decltype(Y)::value;
+        arrive(LEFT2);
+        multiply(I0, X, [&](int s) {
+            read_w(hy, y, s);
+            if (s % 2) fetch_a(s2, k2, 0, a0, s / 2);
+        });
+        multiply(I0, Y, [&](int s) {
+            read_a(1, a1, s);
+            if (s % 2) fetch_w(s2, k2, hx, x, s / 2);
+        });
+        arrive(LEFT2);
         multiply(I1, Y, [&](int s) {
-            read_a(0, na, s);
-            fetch_a(s2, sa, s);
+            read_a(0, a0n, s);
+            if (s % 2) fetch_w(s2, k2, hy, y, s / 2);
         });
         multiply(I1, X, [&](int s) {
-            read_w(y, nw, s);
-            fetch_w(s2, sw, s);
+            read_w(hy, yn, s);
+            if (s % 2) fetch_a(s2, k2, 1, a1, s / 2);
         });
     };
 
@@ -357,9 +367,20 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     int t = map.at(0, blockIdx.x, gridDim.x);
     if (t < 0) return;
     cur = source(t);
-    fetch(cur, 0, sa0, sw0);
-    arrive();
-    fetch(cur, 1, sa1, sw1);
+    auto fetch = [&](auto&& load) {
+        #pragma unroll
+        for (int j = 0; j < 4; j++) load(j);
+    };
+    // in the order in which they are read
+    fetch([&](int j) { fetch_a(cur, 0, 0, sa00, j); });
+    fetch([&](int j) { fetch_w(cur, 0, 0, sw00, j); });
+    fetch([&](int j) { fetch_w(cur, 0, 1, sw10, j); });
+    fetch([&](int j) { fetch_a(cur, 0, 1, sa10, j); });
+    fetch([&](int j) { fetch_a(cur, 1, 0, sa01, j); });
+    fetch([&](int j) { fetch_w(cur, 1, 1, sw11, j); });
+    fetch([&](int j) { fetch_w(cur, 1, 0, sw01, j); });
+    fetch([&](int j) { fetch_a(cur, 1, 1, sa11, j); });
+    arrive(LEFT3);
     while (true) {
         const int t_next = map.at(++i, blockIdx.x, gridDim.x);
         nxt = source(t_next);
@@ -367,16 +388,16 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         // kept them over the epilogue)
         #pragma unroll
         for (int s = 0; s < 8; s++) {
-            read_a(0, sa0, s);
-            read_w(0, sw0, s);
+            read_a(0, sa00, s);
+            read_w(0, sw00, s);
         }
         zero();
         for (int k = 2; k <= steps; k += 2) {
             // the last two steps fetch the next tile's first two
             const Src& s2 = k == steps ? nxt : cur;
             const int k2 = k == steps ? 0 : k;
-            step(I0, I1, sa0, sw0, sa1, sw1, s2, k2);
-            step(I1, I0, sa1, sw1, sa0, sw0, s2, k2 + 1);
+            step(I0, I1, sa00, sa10, sw00, sw10, sa01, sw11, s2, k2);
+            step(I1, I0, sa01, sa11, sw11, sw01, sa00, sw00, s2, k2 + 1);
         }
 
         // lane (g, r): row r of each of 8 groups of 16 rows of a, and of each
