@@ -33,12 +33,7 @@ HIP_FLAGS = [
 # compare and a second exec mask: 6 VALU and 6 SALU per tile), so it is off
 # for kernels.hip.
 KERNEL_FLAGS = ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
-# Norm and rounding of rows; the FP8 product, whose accumulators fill all 256
-# AGPRs: selecting its matrix instructions with VGPR operands first and moving
-# them to AGPRs after register allocation leaves 29 copies in a loop of 128
-# matrix instructions instead of 336.
-LAYER_SOURCES = {"rows": [], "linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1",
-                            "-mllvm", "-disable-machine-licm=1"]}
+LAYER_SOURCES = ["rows", "linear"]   # norm and rounding of rows; the FP8 product
 CXX_FLAGS = ["-O3", "-fPIC", "-std=c++17", "-fopenmp", "-Wall", "-Wextra"]
 
 
@@ -64,8 +59,8 @@ def build(asm: bool = False) -> str:
           "-o", kern_o])
     _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, "encode.hip"), "-o", enc_o])
     layer_o = [os.path.join(BUILD, f"{name}.o") for name in LAYER_SOURCES]
-    for (name, flags), obj in zip(LAYER_SOURCES.items(), layer_o):
-        _run([HIPCC, *HIP_FLAGS, *flags, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj])
+    for name, obj in zip(LAYER_SOURCES, layer_o):
+        _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj])
     if asm:
         _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "--cuda-device-only", "-S",
               os.path.join(CSRC, "kernels.hip"), "-o", os.path.join(BUILD, "kernels.s")])

@@ -176,8 +176,10 @@ __device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
                (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
 }
 
-__device__ __forceinline__ v4f mfma(const v8i& w, const v8i& a, const v4f& c) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ v16f mfma(const v8i& w, const v8i& a, const v16f& c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
 }
 
 // Where a workgroup's tiles lie: the tile sequence takes groups of kGroupM
@@ -223,16 +225,21 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int wm = wave >> 1, wn = wave & 1;
-    const int r = lane & 15, g = lane >> 4;
+    const int r = lane & 31, g = lane >> 5;
     const uint32_t row_bytes = (uint32_t)C;
     const int steps = (int)((C + 2 * kStep - 1) / (2 * kStep)) * 2;   // even
+
+    // Of the 32 x 32 products of an instruction lane (g, r) gets those of a's
+    // row r with w's rows 8 i + 4 g + c (i, c = 0 .. 3) of the operand; w's row
+    // 16 g + 4 i + c is put there, so that a lane's 16 outputs are consecutive.
+    const int wrow = ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
 
     // Loads: one instruction brings 8 rows of 128 bytes, lane l the 16 bytes
     // that belong at position l % 8 of row l / 8.  A row's 16-byte pieces are
     // permuted by an exclusive or with a key of the row, see `frag`.
     const int lrow = wave * 8 + (lane >> 3), lpos = lane & 7;
     const int akey = ((lane >> 4) & 3) | ((wave & 1) << 2);
-    const int wkey = ((lane >> 4) & 1) | ((wave >> 1) << 1);      // and 4 for odd instructions
+    const int wkey = ((lane >> 4) & 1) | ((wave >> 1) << 1) | ((lane >> 5) << 2);
     const uint32_t acol = (uint32_t)(lpos ^ akey) * 16, wcol = (uint32_t)(lpos ^ wkey) * 16;
     const uint32_t lbase = (uint32_t)lrow * row_bytes;
 
@@ -268,53 +275,51 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
                      (uint32_t)((j >> 1) * 128 + h * 64 + (j & 1) * 32) * row_bytes);
     };
     auto fetch_w = [&](const Src& s, int k, int h, uint8_t* unit, int j) {
-        const uint32_t c = (uint32_t)k * kStep + (j & 1 ? wcol ^ 64 : wcol);
+        const uint32_t c = (uint32_t)k * kStep + wcol;
         load_lds(h ? s.w1 : s.w0, unit + opaque_s(wave * 1024) + j * 4096,
                  (c < row_bytes ? lbase + c : kOut) + (uint32_t)j * 32 * row_bytes);
     };
 
-    // Fragments: lane (g, r) takes pieces g and 4 + g of its row.
-    const int key = r >> 1;
-    const uint32_t piece = (uint32_t)(((g ^ key) & 3) | (key & 4)) * 16;
-    uint32_t abase[2], wbase[2];
-    abase[0] = wm * 8192 + r * 128 + piece;
-    wbase[0] = wn * 8192 + (r >> 2) * 2048 + (r & 3) * 128 + piece;
-    abase[1] = abase[0] ^ 64;
-    wbase[1] = wbase[0] ^ 64;
-    // (opaque: otherwise the exclusive or is done, and kept, for every piece)
-    abase[1] = opaque_v(abase[1]);
-    wbase[1] = opaque_v(wbase[1]);
-    v8i fa[8], fw[8];     // 16 rows each; fw[4 h + f]: half h
-    v4f acc[8][8];
+    // Fragments: of each group of 32 rows lane (g, r) takes the 16-byte pieces
+    // g, 2 + g, 4 + g and 6 + g of one, two for each of two products.
+    const int key = (r >> 1) & 7;
+    uint32_t abase[4], wbase[4];
+    #pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint32_t piece = (uint32_t)((2 * q + g) ^ key) * 16;
+        abase[q] = opaque_v((wm * 64 + r) * 128 + piece);
+        wbase[q] = opaque_v((wn * 64 + wrow) * 128 + piece);
+    }
+    v8i fa[4][2], fw[4][2];     // [2 h + group of 32 rows][product]: half h
+    v16f acc[4][4];
     auto zero = [&]() {
         #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 4; i++)
             #pragma unroll
-            for (int j = 0; j < 8; j++) acc[i][j] = v4f{0, 0, 0, 0};
+            for (int j = 0; j < 4; j++)
+                #pragma unroll
+                for (int c = 0; c < 16; c++) acc[i][j][c] = 0.0f;
     };
-    // half s % 2 of fragment s / 2 of a half, s = 0 .. 7
+    // piece s % 4 of group s / 4 of a half, s = 0 .. 7
     auto set = [](v8i& f, int half, const v4u& u) {
         #pragma unroll
         for (int i = 0; i < 4; i++) f[4 * half + i] = (int)u[i];
     };
     auto read_a = [&](int h, const uint8_t* unit, int s) {
-        set(fa[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 2 * 2048 + abase[s % 2]));
+        set(fa[2 * h + s / 4][s % 4 / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 4 * 4096 + abase[s % 4]));
     };
     auto read_w = [&](int h, const uint8_t* unit, int s) {
-        set(fw[4 * h + s / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 2 * 512 + wbase[s % 2]));
+        set(fw[2 * h + s / 4][s % 4 / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 4 * 4096 + wbase[s % 4]));
     };
-    // The 16 products of halves HA and HW in 8 slots of two, each with what
-    // `with` issues for it (LDS reads for the next phase, loads).
+    // The 8 products of halves HA and HW, each with what `with` issues before
+    // it (LDS reads for the next phase, loads).
     auto multiply = [&](auto HA, auto HW, auto&& with) {
         constexpr int ha = decltype(HA)::value, hw = decltype(HW)::value;
         #pragma unroll
         for (int s = 0; s < 8; s++) {
             with(s);
-            #pragma unroll
-            for (int p = 2 * s; p < 2 * s + 2; p++) {
-                v4f& c = acc[4 * ha + p / 4][4 * hw + p % 4];
-                c = mfma(fw[4 * hw + p % 4], fa[4 * ha + p / 4], c);
-            }
+            v16f& c = acc[2 * ha + s % 4 / 2][2 * hw + s % 2];
+            c = mfma(fw[2 * hw + s % 2][s / 4], fa[2 * ha + s % 4 / 2][s / 4], c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -400,32 +405,27 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
             step(I1, I0, sa01, sa11, sw11, sw01, sa00, sw00, s2, k2 + 1);
         }
 
-        // lane (g, r): row r of each of 8 groups of 16 rows of a, and of each
-        // half of w's rows 16 consecutive ones from 64 wn + 16 g on
-        float ws[2][16], bs[2][16];
-        int64_t col[2];
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            col[h] = cur.n0 + (GATED ? 0 : h * kHalf) + wn * 64 + g * 16;
-            columns(e, (GATED && h ? N : 0), col[h], N, ws[h], bs[h]);
-        }
         const bool vec = N % 8 == 0;
         #pragma unroll
-        for (int im = 0; im < 8; im++) {
-            const int64_t m = cur.m0 + wm * 128 + im * 16 + r;
-            if (m >= M) break;
-            const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
+        for (int f = 0; f < (GATED ? 2 : 4); f++) {
+            // 16 consecutive outputs of each of 4 rows
+            const int64_t col = cur.n0 + f / 2 * kHalf + wn * 64 + f % 2 * 32 + g * 16;
+            float ws[16], bs[16], wu[16], bu[16];
+            columns(e, 0, col, N, ws, bs);
+            if (GATED) columns(e, N, col, N, wu, bu);
             #pragma unroll
-            for (int h = 0; h < (GATED ? 1 : 2); h++) {
+            for (int i = 0; i < 4; i++) {
+                const int64_t m = cur.m0 + wm * 128 + i * 32 + r;
+                if (m >= M) break;
+                const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
                 float v[16];
                 #pragma unroll
                 for (int c = 0; c < 16; c++) {
-                    v[c] = acc[im][4 * h + c / 4][c % 4] * sm * ws[h][c] + bs[h][c];
-                    v[c] = activate<ACT>(v[c], e);
-                    if (GATED) v[c] *= acc[im][4 + c / 4][c % 4] * sm * ws[1][c] + bs[1][c];
+                    v[c] = activate<ACT>(acc[i][f][c] * sm * ws[c] + bs[c], e);
+                    if (GATED) v[c] *= acc[i][2 + f % 2][c] * sm * wu[c] + bu[c];
                 }
-                const int64_t o = m * N + col[h];
-                if (vec && col[h] + 16 <= N) {
+                const int64_t o = m * N + col;
+                if (vec && col + 16 <= N) {
                     #pragma unroll
                     for (int b = 0; b < 2; b++) {
                         if (e.residual) {
@@ -442,7 +442,9 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
                         *reinterpret_cast<v4u*>(e.y + o + 8 * b) = u;
                     }
                 } else {
-                    for (int c = 0; c < 16 && col[h] + c < N; c++) {
+                    #pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        if (col + c >= N) break;
                         if (e.residual) v[c] += bf16_lo(e.residual[o + c]);
                         e.y[o + c] = (uint16_t)bf16_pack(v[c], 0.0f);
                     }
