@@ -21,6 +21,11 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 
 constexpr int64_t kMaxCols = int64_t(1) << 22;   // a tile's rows stay below 2^32 bytes
 
+constexpr int kStep = 128;   // columns (bytes) of a step
+// An offset past every tile's bytes (256 rows of kMaxCols: 2^30), also with a
+// row's offset added
+constexpr uint32_t kOut = 0x80000000u;
+
 constexpr float kLog2e = 1.44269504f;
 
 struct Epilogue {
@@ -63,55 +68,40 @@ __device__ __forceinline__ float activate(float v, const Epilogue& e) {
     }
 }
 
-// A wave computes 16 rows of a times 16 outputs; 4 waves of a workgroup take
-// consecutive groups of 16 outputs.  Operands go from memory straight to
-// registers: lane l holds row l % 16 of either and, of each 128 columns,
-// columns 32 (l / 16) .. + 31.  Of the 16 x 16 products, lane l gets those of
-// a's row l % 16 with weight rows 4 (l / 16) .. + 3.
-template <bool GATED, int ACT>
-__global__ __launch_bounds__(256) void linear_kernel(const uint8_t* __restrict__ a,
-                                                     const uint8_t* __restrict__ w, int64_t M,
-                                                     int64_t N, int64_t C, Epilogue e) {
-    const int lane = threadIdx.x & (kLanes - 1);
-    const int r = lane & 15, g = lane >> 4;
-    const int64_t blocks = (N + 63) / 64;   // of 64 outputs, for each 16 rows
-    const int64_t m = blockIdx.x / blocks * 16 + r;
-    const int64_t n0 = (blockIdx.x % blocks * 4 + threadIdx.x / kLanes) * 16;
-    if (n0 >= N) return;
-    const int64_t n = n0 + r < N ? n0 + r : N - 1;   // in bounds; not stored
-    const uint8_t* pa = a + (m < M ? m : M - 1) * C;
-    const uint8_t* pw = w + n * C;
-    const uint8_t* pu = w + (N + n) * C;
-    auto load = [&](const uint8_t* p, int64_t k) {
-        v4u lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-        if (k < C) lo = *reinterpret_cast<const v4u*>(p + k);          // C % 16 == 0
-        if (k + 16 < C) hi = *reinterpret_cast<const v4u*>(p + k + 16);
-        return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
-                   (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    };
-    v4f acc = {0, 0, 0, 0}, up = {0, 0, 0, 0};
-    for (int64_t k = 32 * g; k < C + 32 * g; k += 128) {
-        const v8i av = load(pa, k);
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(load(pw, k), av, acc, 0, 0, 0, 0, 0, 0);
-        if (GATED)
-            up = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(load(pu, k), av, up, 0, 0, 0, 0, 0, 0);
-    }
-    if (m >= M) return;
-    const float sa = e.a_scale ? e.a_scale[m] : 1.0f;
-    for (int i = 0; i < 4; i++) {
-        const int64_t c = n0 + 4 * g + i;
-        if (c >= N) break;
-        auto scaled = [&](float v, int64_t col) {
-            v = v * sa * ((e.w_scale ? e.w_scale[col] : 1.0f) * e.scale);
-            return e.bias ? v + bf16_lo(e.bias[col]) : v;
-        };
-        float v = activate<ACT>(scaled(acc[i], c), e);
-        if (GATED) v *= scaled(up[i], N + c);
-        if (e.residual) v += bf16_lo(e.residual[m * N + c]);
-        e.y[m * N + c] = (uint16_t)bf16_pack(v, 0.0f);
-    }
+constexpr int kNT = 2;   // cache policy: non-temporal
+
+// 16 bytes a lane from memory to LDS, lane l's to lds + 16 l; zeros from
+// offsets out of range.
+template <int POLICY>
+__device__ __forceinline__ void load_lds(const Rsrc& src, uint8_t* lds, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16,
+                                             (int)offset, 0, 0, POLICY);
 }
 
+// Waits until at most N of the wave's loads (those issued last) are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "a 6-bit counter");
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xF70);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Between a wave's writes to LDS and its reads of what other lanes wrote, and
+// back: the hardware keeps a wave's LDS accesses in order, the compiler only
+// those of one lane.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
+    return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
+               (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
 
 // Scale and bias of w's rows first + c .. first + c + CN - 1, of which those
 // with c + i < N exist (the others are repeats of the last).
@@ -143,22 +133,140 @@ __device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_
 }
 
 // ---------------------------------------------------------------------
-// Tiles of 256 rows of a by 256 rows of w, for products with many rows.
+// Few rows of a: w streamed from memory to registers.
 // ---------------------------------------------------------------------
-constexpr int kTile = 256;          // rows of either operand
-constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
-constexpr int kStep = 128;          // columns (bytes) of a step
-constexpr int kUnit = kHalf * kStep;
-constexpr int kTileWaves = 4;
-// An offset past every tile's bytes (kTile * kMaxCols = 2^30), also with a
-// tile's row offset added
-constexpr uint32_t kOut = 0x80000000u;
 
-// 16 bytes a lane from memory to LDS, lane l's to lds + 16 l; zeros from
-// offsets out of range.
-__device__ __forceinline__ void load_lds(const Rsrc& src, uint8_t* lds, uint32_t offset) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16,
-                                             (int)offset, 0, 0, 0);
+// Products of up to 8 MA rows of a.  A workgroup takes 16 NF rows of w (gated:
+// NF / 2 groups of 16 gate rows and the value rows that belong to them); its KW
+// waves share the columns, wave k steps k, k + KW, ... of 128.  Each wave streams
+// its steps through LDS of its own, PIPE steps deep, and waits for its own loads
+// only.  A load brings 8 rows of 128 bytes, whole cache lines; lane l the 16
+// bytes that belong at position l % 8 of row l / 8, a row's pieces permuted by an
+// exclusive or with a key of the row so that 16 rows' reads of a piece touch all
+// banks.  Lane (g, r) then reads, of row r of a group of 16, the pieces g and
+// 4 + g, the same for a and w, and gets of the 16 x 16 products of an
+// instruction those of a's row r with w's rows 4 g .. 4 g + 3.  The waves' sums
+// are added in wave order through LDS.
+template <bool GATED, int ACT, int MA, int NF, int KW, int PIPE>
+__global__ __launch_bounds__(KW * kLanes) void linear_stream_kernel(
+    const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
+    Epilogue e) {
+    constexpr int NO = GATED ? NF / 2 : NF;   // groups of 16 outputs
+    constexpr int MF = (MA + 1) / 2;          // groups of 16 rows of a
+    constexpr int kWave = (MF + NF) * 16 * kStep;   // bytes of a wave's step
+    // (arrays of their own, so that a read waits for its own step's loads only)
+    __shared__ __attribute__((aligned(1024))) uint8_t ring0[KW * kWave], ring1[KW * kWave],
+        ring2[PIPE > 2 ? KW * kWave : 1], ring3[PIPE > 3 ? KW * kWave : 1];
+    __shared__ float part[KW][MF * NF * 4][kLanes];
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int r = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NO);
+    const uint32_t row_bytes = (uint32_t)C;
+    const uint32_t rows = (uint32_t)(N - n0 < 16 * NO ? N - n0 : 16 * NO);
+    const Rsrc asrc = rsrc(a, (uint32_t)M * row_bytes);
+    const Rsrc wsrc = rsrc(w + n0 * C, rows * row_bytes);
+    const Rsrc usrc = rsrc(w + (GATED ? N + n0 : n0) * C, rows * row_bytes);
+    // rows 8 j + lane / 8 of a group: key (row / 2) % 8, another one for odd j
+    const int lrow = lane >> 3, lpos = lane & 7;
+    const uint32_t lcol[2] = {(uint32_t)(lpos ^ (lrow >> 1)) * 16, (uint32_t)(lpos ^ (lrow >> 1) ^ 4) * 16};
+    const uint32_t lbase = (uint32_t)lrow * row_bytes;
+    auto load = [&](int step, uint8_t* ring) {
+        uint8_t* to = ring + wave * kWave;
+        uint32_t o[2];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t c = (uint32_t)step * kStep + lcol[h];
+            o[h] = c < row_bytes ? lbase + c : kOut;
+        }
+        #pragma unroll
+        for (int j = 0; j < 2 * NF; j++)
+            load_lds<kNT>(GATED && j >= 2 * NO ? usrc : wsrc, to + j * 1024,
+                          o[j & 1] + (uint32_t)(GATED ? j % (2 * NO) : j) * 8 * row_bytes);
+        #pragma unroll
+        for (int j = 0; j < MA; j++)
+            load_lds<0>(asrc, to + NF * 2048 + j * 1024, o[j & 1] + (uint32_t)j * 8 * row_bytes);
+    };
+    const uint32_t fbase = (uint32_t)wave * kWave + r * kStep + (uint32_t)(g ^ (r >> 1)) * 16;
+    auto frag = [&](const uint8_t* ring, int i) {   // group i of the step
+        return join(*reinterpret_cast<const v4u*>(ring + i * 2048 + fbase),
+                    *reinterpret_cast<const v4u*>(ring + i * 2048 + (fbase ^ 64)));
+    };
+    v4f acc[MF][NF];
+    #pragma unroll
+    for (int i = 0; i < MF; i++)
+        #pragma unroll
+        for (int j = 0; j < NF; j++) acc[i][j] = v4f{0, 0, 0, 0};
+    auto multiply = [&](int next, uint8_t* ring) {
+        wait_loads<(PIPE - 1) * (2 * NF + MA)>();   // all but the later steps' have come
+        v8i fa[MF], fw[NF];
+        #pragma unroll
+        for (int i = 0; i < NF; i++) fw[i] = frag(ring, i);
+        #pragma unroll
+        for (int i = 0; i < MF; i++) fa[i] = frag(ring, NF + i);
+        #pragma unroll
+        for (int j = 0; j < NF; j++)
+            #pragma unroll
+            for (int i = 0; i < MF; i++)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[j], fa[i], acc[i][j],
+                                                                             0, 0, 0, 0, 0, 0);
+        // (the products have waited for the reads: their slot is free)
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        load(next, ring);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // (steps past the last load zeros)
+    const int steps = (int)((C + kStep - 1) / kStep);
+    load(wave, ring0);
+    load(wave + KW, ring1);
+    if (PIPE > 2) load(wave + 2 * KW, ring2);
+    if (PIPE > 3) load(wave + 3 * KW, ring3);
+    for (int s = wave; s < steps; s += PIPE * KW) {
+        multiply(s + PIPE * KW, ring0);
+        multiply(s + (PIPE + 1) * KW, ring1);
+        if (PIPE > 2) multiply(s + (PIPE + 2) * KW, ring2);
+        if (PIPE > 3) multiply(s + (PIPE + 3) * KW, ring3);
+    }
+    #pragma unroll
+    for (int i = 0; i < MF; i++)
+        #pragma unroll
+        for (int j = 0; j < NF; j++)
+            #pragma unroll
+            for (int c = 0; c < 4; c++) part[wave][(i * NF + j) * 4 + c][lane] = acc[i][j][c];
+    __syncthreads();
+    // one output a thread, consecutive ones along a row of y
+    const int n_rows = (int)M;
+    for (int t = threadIdx.x; t < n_rows * 16 * NO; t += KW * kLanes) {
+        const int m = t / (16 * NO), n = t % (16 * NO);
+        if (n >= (int)rows) continue;
+        auto sum = [&](int j) {   // of group j: w's row n % 16 of it
+            float v = 0.0f;
+            #pragma unroll
+            for (int k = 0; k < KW; k++)
+                v += part[k][(m / 16 * NF + j) * 4 + n % 4][n % 16 / 4 * 16 + m % 16];
+            return v;
+        };
+        const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
+        auto scaled = [&](float v, int64_t col) {
+            v = v * sm * ((e.w_scale ? e.w_scale[col] : 1.0f) * e.scale);
+            return e.bias ? v + bf16_lo(e.bias[col]) : v;
+        };
+        float v = activate<ACT>(scaled(sum(n / 16), n0 + n), e);
+        if (GATED) v *= scaled(sum(NO + n / 16), N + n0 + n);
+        const int64_t o = (int64_t)m * N + n0 + n;
+        if (e.residual) v += bf16_lo(e.residual[o]);
+        e.y[o] = (uint16_t)bf16_pack(v, 0.0f);
+    }
+}
+
+// ---------------------------------------------------------------------
+// Some rows of a: tiles of 32 MI rows of a by 32 NW rows of w.
+// ---------------------------------------------------------------------
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ v16f mfma(const v8i& w, const v8i& a, const v16f& c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
 }
 
 // x, of which the compiler knows nothing any more
@@ -171,23 +279,343 @@ __device__ __forceinline__ uint32_t opaque_v(uint32_t x) {
     return x;
 }
 
-__device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
-    return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
-               (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+// A barrier for which all but each wave's last N loads into LDS have arrived,
+// and its LDS reads (the compiler's own waits cover a wave's own loads only;
+// __syncthreads would wait for all of them).
+template <int N>
+__device__ __forceinline__ void arrive() {
+    static_assert(N < 64, "a 6-bit counter");
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x070);   // vmcnt(N), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-typedef float v16f __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ v16f mfma(const v8i& w, const v8i& a, const v16f& c) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
+// Outputs go through LDS, some rows of W sums of a wave's own (gated: W / 2
+// gates, then their values): a lane's sums lie in a row each, 32 rows to an
+// instruction, and stored from there outputs would be 16-byte writes all over y.
+// 16-byte pieces of a row are permuted by an exclusive or with a key of the row,
+// so that 16 rows' writes of a piece, and a row's reads, touch all banks.
+template <int W>
+__device__ __forceinline__ int staged(int row, int piece) {   // in floats
+    const int key = W >= 64 ? row & 15 : (row >> 1) & 7;
+    return row * W + (piece ^ key) * 4;
 }
+
+__device__ __forceinline__ v4f quad(const v16f& v, int b, float by) {
+    return v4f{v[4 * b] * by, v[4 * b + 1] * by, v[4 * b + 2] * by, v[4 * b + 3] * by};
+}
+
+// What ROWS rows of y (from m0) by W columns (gated W / 2) from c0 need besides
+// the sums, loaded before any of them is stored: loads and stores count as one
+// sequence, and a load between stores would wait for them.  A lane takes eight
+// columns of every 512 / W-th row (gated 1024 / W).
+template <bool GATED, int W>
+struct Columns {
+    float ws[8], bs[8], wu[8], bu[8];
+    __device__ __forceinline__ Columns(const Epilogue& e, int64_t c0, int64_t N) {
+        const int64_t c = c0 + threadIdx.x % kLanes % ((GATED ? W / 2 : W) / 8) * 8;
+        if (c >= N) return;   // (nothing of it is stored)
+        columns(e, 0, c, N, ws, bs);
+        if (GATED) columns(e, N, c, N, wu, bu);
+    }
+};
+
+template <int CW, int ROWS>
+struct Residual {
+    static constexpr int per_row = CW / 8, Q = ROWS * per_row / kLanes;
+    v4u u[Q];
+    __device__ __forceinline__ void load(const Epilogue& e, int64_t m0, int64_t M, int64_t c0, int64_t N) {
+        const int lane = threadIdx.x % kLanes;
+        const int64_t c = c0 + lane % per_row * 8;
+        #pragma unroll
+        for (int q = 0; q < Q; q++) {
+            u[q] = v4u{0, 0, 0, 0};
+            const int64_t m = m0 + q * (kLanes / per_row) + lane / per_row;
+            if (!e.residual || m >= M) continue;
+            const uint16_t* p = e.residual + m * N + c;
+            if (c + 8 <= N) {
+                __builtin_memcpy(&u[q], p, 16);   // rows of y need not be aligned
+            } else {
+                #pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (c + i < N) u[q][i / 2] |= (uint32_t)p[i] << (i % 2 * 16);
+            }
+        }
+    }
+};
+
+template <bool GATED, int ACT, int W, int ROWS>
+__device__ __forceinline__ void store_staged(const float* stage, const Epilogue& e,
+                                             const Columns<GATED, W>& k,
+                                             const Residual<(GATED ? W / 2 : W), ROWS>& res,
+                                             int64_t m0, int64_t M, int64_t c0, int64_t N) {
+    using Res = Residual<(GATED ? W / 2 : W), ROWS>;
+    const int lane = threadIdx.x % kLanes;
+    const int p = lane % Res::per_row * 2;
+    const int64_t c = c0 + p * 4;
+    wave_sync();
+    #pragma unroll
+    for (int q = 0; q < Res::Q; q++) {
+        const int row = q * (kLanes / Res::per_row) + lane / Res::per_row;
+        const int64_t m = m0 + row;
+        float v[8];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const v4f x = *reinterpret_cast<const v4f*>(stage + staged<W>(row, p + h));
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[4 * h + i] = activate<ACT>(x[i] * k.ws[4 * h + i] + k.bs[4 * h + i], e);
+            if constexpr (GATED) {
+                const v4f u = *reinterpret_cast<const v4f*>(stage + staged<W>(row, W / 8 + p + h));
+                #pragma unroll
+                for (int i = 0; i < 4; i++) v[4 * h + i] *= u[i] * k.wu[4 * h + i] + k.bu[4 * h + i];
+            }
+        }
+        if (m >= M || c >= N) continue;
+        if (e.residual) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[2 * i] += bf16_lo(res.u[q][i]);
+                v[2 * i + 1] += bf16_hi(res.u[q][i]);
+            }
+        }
+        const v4u out = {bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]), bf16_pack(v[4], v[5]),
+                         bf16_pack(v[6], v[7])};
+        uint16_t* y = e.y + m * N + c;
+        if (c + 8 <= N) {
+            __builtin_memcpy(y, &out, 16);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (c + i < N) y[i] = (uint16_t)(out[i / 2] >> (i % 2 * 16));
+        }
+    }
+    wave_sync();
+}
+
+// Workgroups run on XCD (block % 8): a permutation of the blocks that gives each
+// XCD a run of neighbours.
+constexpr int kXcds = 8;
+__device__ __forceinline__ int xcd_order(int block, int blocks) {
+    const int xcd = block % kXcds, per = blocks / kXcds, more = blocks % kXcds;
+    return xcd * per + (xcd < more ? xcd : more) + block / kXcds;
+}
+
+struct MidMap {
+    int tiles_m, tiles_n, splits;
+    int64_t Np;       // outputs of a row of partial sums, a multiple of 16
+    float* sums;      // splits > 1: [splits][M][1 or, gated, 2][Np]
+};
+
+// Workgroup: NW waves, each 32 rows of w (gated: 16 gate and 16 value rows) times
+// 32 MI rows of a; `splits` workgroups share a
+// tile's columns and leave 32-bit partial sums.  Each wave loads its own rows of
+// w and its part of a's, PIPE - 1 steps of 128 columns ahead; one barrier a
+// step.  Pieces, keys and banks as in linear_tile_kernel below.
+template <bool GATED, int ACT, int MI, int NW, int PIPE>
+__global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
+    const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
+    MidMap map, Epilogue e) {
+    constexpr int kLoadsA = (4 * MI + NW - 1) / NW;   // of 8 rows; the last ones may be past a's
+    constexpr int kA = kLoadsA * NW * 1024, kW = NW * 32 * kStep;
+    constexpr int kOut16 = GATED ? 8 : 16;      // consecutive outputs of a lane and group
+    constexpr int kLoads = kLoadsA + 4;         // of a wave and step
+    __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW],
+        slot2[PIPE > 2 ? kA + kW : 1], slot3[PIPE > 3 ? kA + kW : 1];
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int r = lane & 31, g = lane >> 5;
+    const uint32_t row_bytes = (uint32_t)C;
+    // the row tiles of a tile of w and their parts are neighbours on one XCD
+    const int item = xcd_order(blockIdx.x, gridDim.x);
+    const int tm = item % map.tiles_m, rest = item / map.tiles_m;
+    const int split = rest % map.splits, tn = rest / map.splits;
+    const int64_t m0 = (int64_t)tm * (32 * MI);
+    const int64_t n0 = ((int64_t)tn * NW + wave) * (GATED ? 16 : 32);   // the wave's
+    const int steps_all = (int)((C + kStep - 1) / kStep);
+    const int k_first = (int)((int64_t)steps_all * split / map.splits);
+    const int k_end = (int)((int64_t)steps_all * (split + 1) / map.splits);
+    const uint32_t col_end = (uint32_t)(k_end * (int64_t)kStep < C ? k_end * (int64_t)kStep : C);
+
+    auto rows = [&](int64_t have, int most) {
+        return (uint32_t)(have < 0 ? 0 : have < most ? have : most) * row_bytes;
+    };
+    const uint32_t wbytes = rows(N - n0, GATED ? 16 : 32);
+    const Rsrc asrc = rsrc(a + m0 * C, rows(M - m0, 32 * MI));
+    const Rsrc wsrc = rsrc(wbytes ? w + n0 * C : w, wbytes);
+    const Rsrc usrc = rsrc(GATED && wbytes ? w + (N + n0) * C : w, GATED ? wbytes : 0);
+    // of w: rows 8 j + lane / 8 of the wave's, key from rows' bits 1, 4 and 2
+    const int lrow = lane >> 3, lpos = lane & 7;
+    const uint32_t acol = (uint32_t)(lpos ^ (lane >> 4)) * 16;   // of an even group of 8 rows
+    uint32_t wcol[2];   // j / 2 even, odd
+    #pragma unroll
+    for (int h = 0; h < 2; h++)
+        wcol[h] = (uint32_t)(lpos ^ (((lane >> 4) & 1) | (h << 1) | ((lane >> 5) << 2))) * 16;
+    auto fetch = [&](int k, uint8_t* slot) {
+        const uint32_t k0 = (uint32_t)(k_first + k) * kStep;
+        const uint32_t to = opaque_s((uint32_t)wave * (32 * kStep));
+        #pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // rows 8 j ..: gated, the gate's 16, then the value's
+            const int row = GATED ? j % 2 * 8 : 8 * j;
+            const uint32_t c = k0 + wcol[j / 2];
+            load_lds<kNT>(GATED && j / 2 ? usrc : wsrc, slot + kA + to + j * 1024,
+                          (c < col_end ? (uint32_t)lrow * row_bytes + c : kOut) + (uint32_t)row * row_bytes);
+        }
+        #pragma unroll
+        for (int j = 0; j < kLoadsA; j++) {
+            const uint32_t group = opaque_s((uint32_t)(j * NW + wave));
+            const uint32_t c = k0 + (acol ^ (group & 1) << 6);
+            load_lds<0>(asrc, slot + group * 1024,
+                        (c < col_end ? (uint32_t)lrow * row_bytes + c : kOut) + group * 8 * row_bytes);
+        }
+    };
+    // Operand row r of w is row 16 b + 4 i + c of its 32 for r = 8 i + 4 b + c, so
+    // that lane (g, r) gets 16 consecutive outputs; gated, 16 (i / 2) + 8 b +
+    // 4 (i % 2) + c: 8 consecutive gates, and their values.
+    const int i4 = r >> 3, b1 = (r >> 2) & 1, c4 = r & 3;
+    const int wrow = GATED ? i4 / 2 * 16 + b1 * 8 + i4 % 2 * 4 + c4 : b1 * 16 + i4 * 4 + c4;
+    const int wkey = ((wrow >> 1) & 1) | ((wrow >> 4) << 1) | (((wrow >> 2) & 1) << 2);
+    uint32_t abase[4], wbase[4];
+    #pragma unroll
+    for (int q = 0; q < 4; q++) {
+        abase[q] = opaque_v(r * kStep + (uint32_t)((2 * q + g) ^ ((r >> 1) & 7)) * 16);
+        wbase[q] = opaque_v(kA + (uint32_t)wave * (32 * kStep) + wrow * kStep +
+                            (uint32_t)((2 * q + g) ^ wkey) * 16);
+    }
+    v16f acc[MI];
+    #pragma unroll
+    for (int i = 0; i < MI; i++)
+        #pragma unroll
+        for (int c = 0; c < 16; c++) acc[i][c] = 0.0f;
+    auto read = [](const uint8_t* p, const uint32_t (&base)[4], int h) {
+        return join(*reinterpret_cast<const v4u*>(p + base[2 * h]),
+                    *reinterpret_cast<const v4u*>(p + base[2 * h + 1]));
+    };
+    // step k in `slot`; the slot of the step before is refilled
+    auto step = [&](int k, uint8_t* slot, uint8_t* before) {
+        arrive<(PIPE - 2) * kLoads>();
+        fetch(k + PIPE - 1, before);
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const v8i fw = read(slot, wbase, h);
+            v8i fa[MI];
+            #pragma unroll
+            for (int i = 0; i < MI; i++) fa[i] = read(slot + i * 4096, abase, h);
+            #pragma unroll
+            for (int i = 0; i < MI; i++) acc[i] = mfma(fw, fa[i], acc[i]);
+        }
+    };
+    fetch(0, slot0);
+    if (PIPE > 2) fetch(1, slot1);
+    if (PIPE > 3) fetch(2, slot2);
+    // (steps past the split's last are zeros)
+    for (int k = 0; k < k_end - k_first; k += PIPE) {
+        if constexpr (PIPE == 2) {
+            step(k, slot0, slot1);
+            step(k + 1, slot1, slot0);
+        } else if constexpr (PIPE == 3) {
+            step(k, slot0, slot2);
+            step(k + 1, slot1, slot0);
+            step(k + 2, slot2, slot1);
+        } else {
+            step(k, slot0, slot3);
+            step(k + 1, slot1, slot0);
+            step(k + 2, slot2, slot1);
+            step(k + 3, slot3, slot2);
+        }
+    }
+    // the slots are free: 4 KiB of them for each wave's sums
+    arrive<0>();
+    if (n0 >= N) return;
+    float* stage = reinterpret_cast<float*>(slot0 + wave * 4096);
+    // gated: the gates' 16 columns, then the values'
+    auto put = [&](int i, float by) {
+        #pragma unroll
+        for (int b = 0; b < 4; b++)
+            *reinterpret_cast<v4f*>(stage + staged<32>(r, GATED ? b / 2 * 4 + g * 2 + b % 2 : g * 4 + b)) =
+                quad(acc[i], b, by);
+    };
+    if (map.splits > 1) {
+        float* to = map.sums + (int64_t)split * M * (GATED ? 2 : 1) * map.Np;
+        #pragma unroll
+        for (int i = 0; i < MI; i++) {
+            put(i, 1.0f);
+            wave_sync();
+            #pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int row = q * 8 + lane / 8, piece = lane % 8;
+                const int64_t m = m0 + i * 32 + row;
+                const v4f v = *reinterpret_cast<const v4f*>(stage + staged<32>(row, piece));
+                const int64_t c = n0 + (GATED ? piece % 4 : piece) * 4;
+                if (m < M && c < map.Np)
+                    *reinterpret_cast<v4f*>(to + (m * (GATED ? 2 : 1) + (GATED ? piece / 4 : 0)) * map.Np + c) = v;
+            }
+            wave_sync();
+        }
+        return;
+    }
+    float sm[MI];
+    Residual<(GATED ? 16 : 32), 32> res[MI];
+    #pragma unroll
+    for (int i = 0; i < MI; i++) {
+        const int64_t m = m0 + i * 32 + r;
+        sm[i] = e.a_scale ? e.a_scale[m < M ? m : M - 1] : 1.0f;
+        res[i].load(e, m0 + i * 32, M, n0, N);
+    }
+    const Columns<GATED, 32> cols(e, n0, N);
+    #pragma unroll
+    for (int i = 0; i < MI; i++) {
+        put(i, sm[i]);
+        store_staged<GATED, ACT, 32, 32>(stage, e, cols, res[i], m0 + i * 32, M, n0, N);
+    }
+}
+
+// y from the splits' sums, added in their order.  A thread takes 4 consecutive
+// outputs.
+template <bool GATED, int ACT>
+__global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M, int64_t N, Epilogue e) {
+    const int64_t quads = map.Np / 4;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = t / quads, n = t % quads * 4;
+    if (m >= M || n >= N) return;
+    const int64_t row = (GATED ? 2 : 1) * map.Np, stride = M * row;
+    const float* p = map.sums + m * row + n;
+    v4f s = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+    for (int k = 0; k < map.splits; k++) {
+        s += *reinterpret_cast<const v4f*>(p + k * stride);
+        if (GATED) u += *reinterpret_cast<const v4f*>(p + k * stride + map.Np);
+    }
+    float ws[4], bs[4], wu[4], bu[4];
+    columns(e, 0, n, N, ws, bs);
+    if (GATED) columns(e, N, n, N, wu, bu);
+    const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
+    #pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (n + i >= N) break;
+        float v = activate<ACT>(s[i] * sm * ws[i] + bs[i], e);
+        if (GATED) v *= u[i] * sm * wu[i] + bu[i];
+        if (e.residual) v += bf16_lo(e.residual[m * N + n + i]);
+        e.y[m * N + n + i] = (uint16_t)bf16_pack(v, 0.0f);
+    }
+}
+
+// ---------------------------------------------------------------------
+// Tiles of 256 rows of a by 256 rows of w, for products with many rows.
+// ---------------------------------------------------------------------
+constexpr int kTile = 256;          // rows of either operand
+constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
+constexpr int kUnit = kHalf * kStep;
+constexpr int kTileWaves = 4;
 
 // Where a workgroup's tiles lie: the tile sequence takes groups of kGroupM
 // tiles of a's rows, in each of them w's tiles in order and the group's row
 // tiles innermost; an eighth of the sequence goes to each of the 8 XCDs
 // (workgroup b runs on XCD b % 8), so that the tiles an XCD works on at a time
 // share their rows of a and w in its L2.
-constexpr int kXcds = 8;
 constexpr int kGroupM = 8;
 
 struct TileMap {
@@ -222,6 +650,7 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     // that a read does not need): s<operand><half><step % 2>
     __shared__ __attribute__((aligned(1024))) uint8_t sa00[kUnit], sa10[kUnit], sw00[kUnit], sw10[kUnit];
     __shared__ __attribute__((aligned(1024))) uint8_t sa01[kUnit], sa11[kUnit], sw01[kUnit], sw11[kUnit];
+    __shared__ __attribute__((aligned(1024))) float out_stage[kTileWaves][32 * 64];
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int wm = wave >> 1, wn = wave & 1;
@@ -270,13 +699,13 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     // 128, w's half h rows 128 h ...
     auto fetch_a = [&](const Src& s, int k, int h, uint8_t* unit, int j) {
         const uint32_t c = (uint32_t)k * kStep + acol;
-        load_lds(s.a, unit + opaque_s(wave * 1024) + j * 4096,
+        load_lds<0>(s.a, unit + opaque_s(wave * 1024) + j * 4096,
                  (c < row_bytes ? lbase + c : kOut) +
                      (uint32_t)((j >> 1) * 128 + h * 64 + (j & 1) * 32) * row_bytes);
     };
     auto fetch_w = [&](const Src& s, int k, int h, uint8_t* unit, int j) {
         const uint32_t c = (uint32_t)k * kStep + wcol;
-        load_lds(h ? s.w1 : s.w0, unit + opaque_s(wave * 1024) + j * 4096,
+        load_lds<0>(h ? s.w1 : s.w0, unit + opaque_s(wave * 1024) + j * 4096,
                  (c < row_bytes ? lbase + c : kOut) + (uint32_t)j * 32 * row_bytes);
     };
 
@@ -325,20 +754,6 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     };
     constexpr std::integral_constant<int, 0> I0{};
     constexpr std::integral_constant<int, 1> I1{};
-    // A barrier for which all but each wave's last LEFT loads into LDS have
-    // arrived, and its LDS reads (the compiler's own waits cover a wave's own
-    // loads only; __syncthreads would wait for all of them).
-    auto arrive = [](auto LEFT) {
-        constexpr int n = decltype(LEFT)::value;
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 0x070);   // vmcnt(n), lgkmcnt(0)
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    constexpr std::integral_constant<int, 16> LEFT2{};   // the loads of two half steps
-    constexpr std::integral_constant<int, 24> LEFT3{};
     // A step in two halves, on its units a0, a1, x, y (w's halves X and Y) and
     // the next step's a0n, yn; a's half 0 and w's half X are in registers.  Each
     // half reads two units and refills the two that the half before has read
@@ -348,7 +763,7 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     auto step = [&](auto X, auto Y, uint8_t* a0, uint8_t* a1, uint8_t* x, uint8_t* y, uint8_t* a0n,
                     uint8_t* yn, const Src& s2, int k2) {
         constexpr int hx = decltype(X)::value, hy = decltype(Y)::value;
-        arrive(LEFT2);
+        arrive<16>();
         multiply(I0, X, [&](int s) {
             read_w(hy, y, s);
             if (s % 2) fetch_a(s2, k2, 0, a0, s / 2);
@@ -357,7 +772,7 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
             read_a(1, a1, s);
             if (s % 2) fetch_w(s2, k2, hx, x, s / 2);
         });
-        arrive(LEFT2);
+        arrive<16>();
         multiply(I1, Y, [&](int s) {
             read_a(0, a0n, s);
             if (s % 2) fetch_w(s2, k2, hy, y, s / 2);
@@ -385,7 +800,7 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     fetch([&](int j) { fetch_w(cur, 1, 1, sw11, j); });
     fetch([&](int j) { fetch_w(cur, 1, 0, sw01, j); });
     fetch([&](int j) { fetch_a(cur, 1, 1, sa11, j); });
-    arrive(LEFT3);
+    arrive<24>();
     while (true) {
         const int t_next = map.at(++i, blockIdx.x, gridDim.x);
         nxt = source(t_next);
@@ -405,56 +820,43 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
             step(I1, I0, sa01, sa11, sw11, sw01, sa00, sw00, s2, k2 + 1);
         }
 
-        const bool vec = N % 8 == 0;
+        float* stage = out_stage[wave];
+        // Lane (g, r) has, of each 32 of w's rows (f), 16 consecutive sums of row
+        // r.  32 rows by a half's 64 columns at a time, or gated 16 rows by 64
+        // gates and their values.
+        constexpr int W = GATED ? 128 : 64, ROWS = GATED ? 16 : 32;
+        float sm[4];
         #pragma unroll
-        for (int f = 0; f < (GATED ? 2 : 4); f++) {
-            // 16 consecutive outputs of each of 4 rows
-            const int64_t col = cur.n0 + f / 2 * kHalf + wn * 64 + f % 2 * 32 + g * 16;
-            float ws[16], bs[16], wu[16], bu[16];
-            columns(e, 0, col, N, ws, bs);
-            if (GATED) columns(e, N, col, N, wu, bu);
+        for (int i = 0; i < 4; i++) {
+            const int64_t m = cur.m0 + wm * 128 + i * 32 + r;
+            sm[i] = e.a_scale ? e.a_scale[m < M ? m : M - 1] : 1.0f;
+        }
+        #pragma unroll
+        for (int h = 0; h < (GATED ? 1 : 2); h++) {
+            const int64_t c0 = cur.n0 + h * kHalf + wn * 64, first = cur.m0 + wm * 128;
+            Residual<64, ROWS> res[128 / ROWS];
             #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t m = cur.m0 + wm * 128 + i * 32 + r;
-                if (m >= M) break;
-                const float sm = e.a_scale ? e.a_scale[m] : 1.0f;
-                float v[16];
-                #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    v[c] = activate<ACT>(acc[i][f][c] * sm * ws[c] + bs[c], e);
-                    if (GATED) v[c] *= acc[i][2 + f % 2][c] * sm * wu[c] + bu[c];
-                }
-                const int64_t o = m * N + col;
-                if (vec && col + 16 <= N) {
+            for (int i = 0; i < 128 / ROWS; i++) res[i].load(e, first + i * ROWS, M, c0, N);
+            const Columns<GATED, W> cols(e, c0, N);
+            #pragma unroll
+            for (int i = 0; i < 128 / ROWS; i++) {
+                const int group = i * ROWS / 32;
+                if (!GATED || r / 16 == i % 2) {
                     #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        if (e.residual) {
-                            const v4u u = *reinterpret_cast<const v4u*>(e.residual + o + 8 * b);
-                            #pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                v[8 * b + 2 * c] += bf16_lo(u[c]);
-                                v[8 * b + 2 * c + 1] += bf16_hi(u[c]);
-                            }
-                        }
-                        v4u u;
+                    for (int f = 0; f < W / 32; f++)
                         #pragma unroll
-                        for (int c = 0; c < 4; c++) u[c] = bf16_pack(v[8 * b + 2 * c], v[8 * b + 2 * c + 1]);
-                        *reinterpret_cast<v4u*>(e.y + o + 8 * b) = u;
-                    }
-                } else {
-                    #pragma unroll
-                    for (int c = 0; c < 16; c++) {
-                        if (col + c >= N) break;
-                        if (e.residual) v[c] += bf16_lo(e.residual[o + c]);
-                        e.y[o + c] = (uint16_t)bf16_pack(v[c], 0.0f);
-                    }
+                        for (int b = 0; b < 4; b++)
+                            *reinterpret_cast<v4f*>(stage + staged<W>(r % ROWS, f * 8 + g * 4 + b)) =
+                                quad(acc[group][2 * h + f], b, sm[group]);
                 }
+                store_staged<GATED, ACT, W, ROWS>(stage, e, cols, res[i], first + i * ROWS, M, c0, N);
             }
         }
         if (t_next < 0) break;
         t = t_next;
         cur = nxt;
     }
+    wait_loads<0>();
 }
 
 // f(gated, activation form) with both as types
@@ -468,6 +870,50 @@ void for_kind(bool gated, int act, F&& f) {
     if (gated) with(std::true_type{}); else with(std::false_type{});
 }
 
+template <int V>
+constexpr std::integral_constant<int, V> kInt{};
+
+// How a product is computed.
+enum Kind { kStream, kMid, kTiles };
+struct Plan {
+    Kind kind;
+    int few;        // kStream: few rows of w, one group of 16 a workgroup
+    int mi, nw;     // kMid: 32 mi rows of a, 32 nw rows of w
+    int splits;     // kMid
+    int64_t tiles_m, tiles_n, Np;
+    int64_t bytes;  // of partial sums
+};
+
+Plan plan(int64_t M, int64_t N, int64_t C, bool gated, int cus) {
+    Plan p = {};
+    auto parts = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+    const int64_t halves = gated ? 2 : 1;
+    p.splits = 1;
+    if (M <= 32) {
+        p.kind = kStream;
+        p.few = !gated && parts(N, 32) < cus;
+        return p;
+    }
+    if (M <= 512) {
+        p.kind = kMid;
+        p.mi = M <= 64 ? 2 : 4;
+        p.nw = 4;
+    } else {
+        p.kind = kTiles;
+        p.mi = p.nw = 0;
+    }
+    //PLAN
+    const int64_t rows_m = p.kind == kTiles ? kTile : 32 * p.mi;
+    const int64_t rows_w = p.kind == kTiles ? kTile : 32 * p.nw;
+    p.tiles_m = parts(M, rows_m);
+    p.tiles_n = parts(N, rows_w / halves);
+    if (p.kind == kMid && p.splits > 1) {
+        p.Np = parts(N, 16) * 16;
+        p.bytes = p.splits * M * halves * p.Np * 4;
+    }
+    return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -478,7 +924,7 @@ int tans_fp8_linear_workspace(int64_t M, int64_t R, int64_t C, int32_t gated, in
         return fail(TANS_EINVAL, "linear: need M >= 0 and R >= 1 below 2^31, R even if gated");
     if (C < 16 || C % 16 || C > kMaxCols)
         return fail(TANS_EINVAL, "linear: C must be a multiple of 16, 16 .. 2^22");
-    *bytes = 0;
+    *bytes = M ? plan(M, gated ? R / 2 : R, C, gated, tans_internal_cu_count()).bytes : 0;
     return TANS_OK;
 }
 
@@ -499,6 +945,8 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
     if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return fail(TANS_EINVAL, "linear: workspace too small, null or misaligned (16 bytes)");
     const int64_t N = gated ? R / 2 : R;
+    const int cus = tans_internal_cu_count();
+    if (cus <= 0) return fail(TANS_EHIP, "linear: cannot query the device's CU count");
     const float tanh_c1 = 2.0f * 0.79788456f * kLog2e;   // 2 sqrt(2 / pi)
     const bool tanh_form = activation == TANS_ACT_GELU_TANH;
     const Epilogue e = {a_scale, w_scale, (const uint16_t*)bias, (const uint16_t*)residual,
@@ -507,30 +955,50 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
                         tanh_form ? tanh_c1 : kLog2e, tanh_form ? 0.044715f * tanh_c1 : 0.0f};
     const int act = activation == TANS_ACT_GELU ? kErf
                     : activation == TANS_ACT_SILU || tanh_form ? kSigmoid : kClip;
-    if (M > 128) {
-        const TileMap map = {(int)((M + kTile - 1) / kTile), (int)((N + (gated ? kHalf : kTile) - 1) / (gated ? kHalf : kTile))};
-        const int64_t tiles = (int64_t)map.tiles_m * map.tiles_n;
-        const int cus = tans_internal_cu_count();
-        auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, cus)), dim3(256), 0,
-                               (hipStream_t)stream, (const uint8_t*)a, (const uint8_t*)w, M, N, C, map, e);
-        };
-        for_kind(gated, act, [&](auto G, auto A) {
-            launch(linear_tile_kernel<decltype(G)::value, decltype(A)::value>);
-        });
-        return hip_check(hipGetLastError(), "linear_tile_kernel launch");
-    }
-    const int64_t blocks = (N + 63) / 64 * ((M + 15) / 16);
-    if (blocks > UINT32_MAX / 256) return fail(TANS_EINVAL, "linear: too many outputs for one call");
-    const dim3 grid((unsigned)blocks);
-    auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const uint8_t*)a,
-                           (const uint8_t*)w, M, N, C, e);
+    const Plan p = plan(M, N, C, gated, cus);
+    const uint8_t *a8 = (const uint8_t*)a, *w8 = (const uint8_t*)w;
+    const hipStream_t st = (hipStream_t)stream;
+    auto launch = [&](auto kernel, int64_t blocks, int threads, auto... args) {
+        if (blocks > INT32_MAX / threads) return fail(TANS_EINVAL, "linear: too many outputs for one call");
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, args...);
+        return hip_check(hipGetLastError(), "linear kernel launch");
     };
+    int out = TANS_OK;
     for_kind(gated, act, [&](auto G, auto A) {
-        launch(linear_kernel<decltype(G)::value, decltype(A)::value>);
+        constexpr bool g = decltype(G)::value;
+        constexpr int ac = decltype(A)::value;
+        auto stream_rows = [&](auto MA) {
+            constexpr int ma = decltype(MA)::value;
+            const int64_t wide = (N + (g ? 16 : 32) - 1) / (g ? 16 : 32);
+            if constexpr (!g) {
+                if (p.few) {
+                    out = launch(linear_stream_kernel<g, ac, ma, 1, 4, 4>, (N + 15) / 16, 256, a8, w8, M, N, C, e);
+                    return;
+                }
+            }
+            out = launch(linear_stream_kernel<g, ac, ma, 2, 4, 2>, wide, 256, a8, w8, M, N, C, e);
+        };
+        if (p.kind == kStream) {
+            if (M <= 8) stream_rows(kInt<1>);
+            else if (M <= 16) stream_rows(kInt<2>);
+            else stream_rows(kInt<4>);
+        } else if (p.kind == kMid) {
+            const MidMap map = {(int)p.tiles_m, (int)p.tiles_n, p.splits, p.Np, (float*)workspace};
+            const int64_t blocks = p.tiles_m * p.tiles_n * p.splits;
+            auto mid = [&](auto MI, auto NW) {
+                constexpr int mi = decltype(MI)::value, nw = decltype(NW)::value;
+                out = launch(linear_mid_kernel<g, ac, mi, nw, 3>, blocks, nw * kLanes, a8, w8, M, N, C, map, e);
+            };
+            //MID
+            if (p.mi == 2) mid(kInt<2>, kInt<4>); else mid(kInt<4>, kInt<4>);
+            if (out == TANS_OK && p.splits > 1)
+                out = launch(linear_join_kernel<g, ac>, (M * (p.Np / 4) + 255) / 256, 256, map, M, N, e);
+        } else {
+            const TileMap map = {(int)p.tiles_m, (int)p.tiles_n};
+            out = launch(linear_tile_kernel<g, ac>, std::min<int64_t>(p.tiles_m * p.tiles_n, cus), 256, a8, w8, M, N, C, map, e);
+        }
     });
-    return hip_check(hipGetLastError(), "linear_kernel launch");
+    return out;
 }
 
 }  // extern "C"
