@@ -350,7 +350,8 @@ int tans_fp8_quantize_rows(const void* x, int64_t M, int64_t D, void* q, float* 
  *   y[m][n] = act(v[m][n]) + residual[m][n]                      (N = R)
  *   gated: y[m][j] = act(v[m][j]) * v[m][R / 2 + j] + residual[m][j]  (N = R / 2)
  * fp32 accumulation in a fixed order, one rounding to bf16 (nearest even).
- *   a          E4M3FN [M, C]; w E4M3FN [R, C]; C a multiple of 16, 16 .. 2^22
+ *   a          E4M3FN [M, C]; w E4M3FN [R, C]; C a multiple of 16, 16 .. 2^22,
+ *              R in 1 .. 2^27 (even if gated)
  *   a_scale    float [M] or NULL (1); w_scale float [R] or NULL (1)
  *   bias       bf16 [R] or NULL; residual bf16 [M, N] or NULL
  *   activation TANS_ACT_*

@@ -19,6 +19,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 
+constexpr int64_t kMaxRows = int64_t(1) << 27;   // of w: eight rows of y stay below 2^32 bytes
 constexpr int64_t kMaxCols = int64_t(1) << 22;   // a tile's rows stay below 2^32 bytes
 
 constexpr int kStep = 128;   // columns (bytes) of a step
@@ -93,9 +94,11 @@ __device__ __forceinline__ void wait_loads() {
 // back: the hardware keeps a wave's LDS accesses in order, the compiler only
 // those of one lane.
 __device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_sched_barrier(0);   // (registers for one chunk at a time)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
@@ -105,7 +108,7 @@ __device__ __forceinline__ v8i join(const v4u& lo, const v4u& hi) {
 
 // Scale and bias of w's rows first + c .. first + c + CN - 1, of which those
 // with c + i < N exist (the others are repeats of the last).
-template <int CN>
+template <int CN, bool WHOLE = false>
 __device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_t c, int64_t N,
                                         float (&ws)[CN], float (&bs)[CN]) {
     #pragma unroll
@@ -114,7 +117,7 @@ __device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_
         bs[i] = 0.0f;
     }
     uint16_t b[CN];
-    if (c + CN <= N) {
+    if (WHOLE || c + CN <= N) {
         if (e.w_scale) __builtin_memcpy(ws, e.w_scale + first + c, sizeof(ws));
         if (e.bias) __builtin_memcpy(b, e.bias + first + c, sizeof(b));
     } else {
@@ -308,18 +311,21 @@ __device__ __forceinline__ v4f quad(const v16f& v, int b, float by) {
     return v4f{v[4 * b] * by, v[4 * b + 1] * by, v[4 * b + 2] * by, v[4 * b + 3] * by};
 }
 
-// What ROWS rows of y (from m0) by W columns (gated W / 2) from c0 need besides
+// What W columns (gated W / 2) from c0 on and ROWS rows from m0 on need besides
 // the sums, loaded before any of them is stored: loads and stores count as one
 // sequence, and a load between stores would wait for them.  A lane takes eight
-// columns of every 512 / W-th row (gated 1024 / W).
+// columns of every 512 / W-th row (gated 1024 / W).  WHOLE: all of them exist,
+// and nothing is masked (a masked load or store ends a run of code in which the
+// compiler can leave loads under way).
 template <bool GATED, int W>
 struct Columns {
     float ws[8], bs[8], wu[8], bu[8];
-    __device__ __forceinline__ Columns(const Epilogue& e, int64_t c0, int64_t N) {
-        const int64_t c = c0 + threadIdx.x % kLanes % ((GATED ? W / 2 : W) / 8) * 8;
-        if (c >= N) return;   // (nothing of it is stored)
-        columns(e, 0, c, N, ws, bs);
-        if (GATED) columns(e, N, c, N, wu, bu);
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const Epilogue& e, int lane, int64_t c0, int64_t N) {
+        const int64_t c = c0 + lane % ((GATED ? W / 2 : W) / 8) * 8;
+        if (!WHOLE && c >= N) return;   // (nothing of it is stored)
+        columns<8, WHOLE>(e, 0, c, N, ws, bs);
+        if (GATED) columns<8, WHOLE>(e, N, c, N, wu, bu);
     }
 };
 
@@ -327,35 +333,37 @@ template <int CW, int ROWS>
 struct Residual {
     static constexpr int per_row = CW / 8, Q = ROWS * per_row / kLanes;
     v4u u[Q];
-    __device__ __forceinline__ void load(const Epilogue& e, int64_t m0, int64_t M, int64_t c0, int64_t N) {
-        const int lane = threadIdx.x % kLanes;
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const Epilogue& e, int lane, int64_t m0, int64_t M, int64_t c0,
+                                         int64_t N) {
         const int64_t c = c0 + lane % per_row * 8;
+        const uint32_t mine = (uint32_t)(lane / per_row) * (uint32_t)N + lane % per_row * 8;
         #pragma unroll
         for (int q = 0; q < Q; q++) {
-            u[q] = v4u{0, 0, 0, 0};
+            // (a uniform part and 32 bits a lane)
+            const uint16_t* p = e.residual + (m0 + q * (kLanes / per_row)) * N + c0 + mine;
             const int64_t m = m0 + q * (kLanes / per_row) + lane / per_row;
-            if (!e.residual || m >= M) continue;
-            const uint16_t* p = e.residual + m * N + c;
-            if (c + 8 <= N) {
-                __builtin_memcpy(&u[q], p, 16);   // rows of y need not be aligned
+            if (WHOLE || (m < M && c + 8 <= N)) {
+                __builtin_memcpy(&u[q], p, 16);   // (rows of y need not be aligned)
             } else {
+                u[q] = v4u{0, 0, 0, 0};
                 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (c + i < N) u[q][i / 2] |= (uint32_t)p[i] << (i % 2 * 16);
+                    if (m < M && c + i < N) u[q][i / 2] |= (uint32_t)p[i] << (i % 2 * 16);
             }
         }
     }
 };
 
-template <bool GATED, int ACT, int W, int ROWS>
+template <bool GATED, int ACT, int W, int ROWS, bool WHOLE>
 __device__ __forceinline__ void store_staged(const float* stage, const Epilogue& e,
                                              const Columns<GATED, W>& k,
                                              const Residual<(GATED ? W / 2 : W), ROWS>& res,
-                                             int64_t m0, int64_t M, int64_t c0, int64_t N) {
+                                             int lane, int64_t m0, int64_t M, int64_t c0, int64_t N) {
     using Res = Residual<(GATED ? W / 2 : W), ROWS>;
-    const int lane = threadIdx.x % kLanes;
     const int p = lane % Res::per_row * 2;
     const int64_t c = c0 + p * 4;
+    const uint32_t mine = (uint32_t)(lane / Res::per_row) * (uint32_t)N + p * 4;
     wave_sync();
     #pragma unroll
     for (int q = 0; q < Res::Q; q++) {
@@ -374,7 +382,6 @@ __device__ __forceinline__ void store_staged(const float* stage, const Epilogue&
                 for (int i = 0; i < 4; i++) v[4 * h + i] *= u[i] * k.wu[4 * h + i] + k.bu[4 * h + i];
             }
         }
-        if (m >= M || c >= N) continue;
         if (e.residual) {
             #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -384,13 +391,13 @@ __device__ __forceinline__ void store_staged(const float* stage, const Epilogue&
         }
         const v4u out = {bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]), bf16_pack(v[4], v[5]),
                          bf16_pack(v[6], v[7])};
-        uint16_t* y = e.y + m * N + c;
-        if (c + 8 <= N) {
+        uint16_t* y = e.y + (m0 + q * (kLanes / Res::per_row)) * N + c0 + mine;
+        if (WHOLE || (m < M && c + 8 <= N)) {
             __builtin_memcpy(y, &out, 16);
         } else {
             #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (c + i < N) y[i] = (uint16_t)(out[i / 2] >> (i % 2 * 16));
+                if (m < M && c + i < N) y[i] = (uint16_t)(out[i / 2] >> (i % 2 * 16));
         }
     }
     wave_sync();
@@ -559,19 +566,28 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
         return;
     }
     float sm[MI];
-    Residual<(GATED ? 16 : 32), 32> res[MI];
     #pragma unroll
     for (int i = 0; i < MI; i++) {
         const int64_t m = m0 + i * 32 + r;
         sm[i] = e.a_scale ? e.a_scale[m < M ? m : M - 1] : 1.0f;
-        res[i].load(e, m0 + i * 32, M, n0, N);
     }
-    const Columns<GATED, 32> cols(e, n0, N);
-    #pragma unroll
-    for (int i = 0; i < MI; i++) {
-        put(i, sm[i]);
-        store_staged<GATED, ACT, 32, 32>(stage, e, cols, res[i], m0 + i * 32, M, n0, N);
-    }
+    auto finish = [&](auto WHOLE) {
+        constexpr bool whole = decltype(WHOLE)::value;
+        Columns<GATED, 32> cols;
+        cols.template load<whole>(e, lane, n0, N);
+        Residual<(GATED ? 16 : 32), 32> res[MI];
+        if (e.residual) {
+            #pragma unroll
+            for (int i = 0; i < MI; i++) res[i].template load<whole>(e, lane, m0 + i * 32, M, n0, N);
+        }
+        #pragma unroll
+        for (int i = 0; i < MI; i++) {
+            put(i, sm[i]);
+            store_staged<GATED, ACT, 32, 32, whole>(stage, e, cols, res[i], lane, m0 + i * 32, M, n0, N);
+        }
+    };
+    if (m0 + MI * 32 <= M && n0 + (GATED ? 16 : 32) <= N) finish(std::true_type{});
+    else finish(std::false_type{});
 }
 
 // y from the splits' sums, added in their order.  A thread takes 4 consecutive
@@ -822,35 +838,46 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
 
         float* stage = out_stage[wave];
         // Lane (g, r) has, of each 32 of w's rows (f), 16 consecutive sums of row
-        // r.  32 rows by a half's 64 columns at a time, or gated 16 rows by 64
-        // gates and their values.
-        constexpr int W = GATED ? 128 : 64, ROWS = GATED ? 16 : 32;
+        // r.  32 rows at a time by a half's 64 columns, or gated by 32 gates and
+        // their values.
+        const int64_t first = cur.m0 + wm * 128;
+        // (opaque: else the lane's addresses are kept, and spilled, over the loop)
+        const int ln = (int)opaque_v((uint32_t)lane), er = ln & 31, eg = ln >> 5;
         float sm[4];
         #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int64_t m = cur.m0 + wm * 128 + i * 32 + r;
+            const int64_t m = first + i * 32 + er;
             sm[i] = e.a_scale ? e.a_scale[m < M ? m : M - 1] : 1.0f;
         }
-        #pragma unroll
-        for (int h = 0; h < (GATED ? 1 : 2); h++) {
-            const int64_t c0 = cur.n0 + h * kHalf + wn * 64, first = cur.m0 + wm * 128;
-            Residual<64, ROWS> res[128 / ROWS];
-            #pragma unroll
-            for (int i = 0; i < 128 / ROWS; i++) res[i].load(e, first + i * ROWS, M, c0, N);
-            const Columns<GATED, W> cols(e, c0, N);
-            #pragma unroll
-            for (int i = 0; i < 128 / ROWS; i++) {
-                const int group = i * ROWS / 32;
-                if (!GATED || r / 16 == i % 2) {
-                    #pragma unroll
-                    for (int f = 0; f < W / 32; f++)
-                        #pragma unroll
-                        for (int b = 0; b < 4; b++)
-                            *reinterpret_cast<v4f*>(stage + staged<W>(r % ROWS, f * 8 + g * 4 + b)) =
-                                quad(acc[group][2 * h + f], b, sm[group]);
-                }
-                store_staged<GATED, ACT, W, ROWS>(stage, e, cols, res[i], first + i * ROWS, M, c0, N);
+        // part: w's half, or gated the first or second 32 of the wave's outputs
+        auto finish = [&](auto PART, auto WHOLE) {
+            constexpr int part = decltype(PART)::value;
+            constexpr bool whole = decltype(WHOLE)::value;
+            const int64_t c0 = cur.n0 + wn * 64 + part * (GATED ? 32 : kHalf);
+            Residual<(GATED ? 32 : 64), 32> res[4];
+            if (e.residual) {
+                #pragma unroll
+                for (int i = 0; i < 4; i++) res[i].template load<whole>(e, ln, first + i * 32, M, c0, N);
             }
+            Columns<GATED, 64> cols;
+            cols.template load<whole>(e, ln, c0, N);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                #pragma unroll
+                for (int f = 0; f < 2; f++)
+                    #pragma unroll
+                    for (int b = 0; b < 4; b++)
+                        *reinterpret_cast<v4f*>(stage + staged<64>(er, f * 8 + eg * 4 + b)) =
+                            quad(acc[i][GATED ? 2 * f + part : 2 * part + f], b, sm[i]);
+                store_staged<GATED, ACT, 64, 32, whole>(stage, e, cols, res[i], ln, first + i * 32, M, c0, N);
+            }
+        };
+        if (first + 128 <= M && cur.n0 + (GATED ? 0 : kHalf) + wn * 64 + 64 <= N) {
+            finish(I0, std::true_type{});
+            finish(I1, std::true_type{});
+        } else {
+            finish(I0, std::false_type{});
+            finish(I1, std::false_type{});
         }
         if (t_next < 0) break;
         t = t_next;
@@ -920,8 +947,8 @@ extern "C" {
 
 int tans_fp8_linear_workspace(int64_t M, int64_t R, int64_t C, int32_t gated, int64_t* bytes) {
     if (!bytes) return fail(TANS_EINVAL, "linear: null pointer");
-    if (M < 0 || R < 1 || M > INT32_MAX || R > INT32_MAX || (gated && R % 2))
-        return fail(TANS_EINVAL, "linear: need M >= 0 and R >= 1 below 2^31, R even if gated");
+    if (M < 0 || R < 1 || M > INT32_MAX || R > kMaxRows || (gated && R % 2))
+        return fail(TANS_EINVAL, "linear: need M >= 0 below 2^31 and R in 1 .. 2^27, even if gated");
     if (C < 16 || C % 16 || C > kMaxCols)
         return fail(TANS_EINVAL, "linear: C must be a multiple of 16, 16 .. 2^22");
     *bytes = M ? plan(M, gated ? R / 2 : R, C, gated, tans_internal_cu_count()).bytes : 0;
