@@ -22,6 +22,9 @@ using namespace tans_linear;
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 
+template <int V>
+constexpr std::integral_constant<int, V> kInt{};
+
 constexpr int64_t kMaxRows = int64_t(1) << 27;   // of w: eight rows of y stay below 2^32 bytes
 constexpr int64_t kMaxCols = int64_t(1) << 22;   // a tile's rows stay below 2^32 bytes
 
@@ -659,36 +662,56 @@ struct TileMap {
     }
 };
 
-template <bool GATED, int ACT>
+// GY: groups of 32 rows of w's second half that a wave takes (2, or 1 for tiles
+// of 192 rows of w).
+template <bool GATED, int ACT, int GY>
 __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
     TileMap map, Epilogue e) {
     // Two steps' operands, each in units of its own (128 rows, 16 KiB; the
     // compiler tells loads into different arrays apart, and waits for none
     // that a read does not need): s<operand><half><step % 2>
-    __shared__ __attribute__((aligned(1024))) uint8_t sa00[kUnit], sa10[kUnit], sw00[kUnit], sw10[kUnit];
-    __shared__ __attribute__((aligned(1024))) uint8_t sa01[kUnit], sa11[kUnit], sw01[kUnit], sw11[kUnit];
+    __shared__ __attribute__((aligned(1024))) uint8_t sa00[kUnit], sa10[kUnit], sw00[kUnit], sw10[kUnit * GY / 2];
+    __shared__ __attribute__((aligned(1024))) uint8_t sa01[kUnit], sa11[kUnit], sw01[kUnit], sw11[kUnit * GY / 2];
     __shared__ __attribute__((aligned(1024))) float out_stage[kTileWaves][32 * 64];
+    static_assert(GY == 2 || (GY == 1 && !GATED), "a gated tile's halves belong together");
+    constexpr int kWide = kHalf + 64 * GY;      // rows of w
+    constexpr int kW0 = 4, kW1 = 2 * GY;        // loads of a wave for w's halves; a's are 4
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int wm = wave >> 1, wn = wave & 1;
-    const int r = lane & 31, g = lane >> 5;
     const uint32_t row_bytes = (uint32_t)C;
     const int steps = (int)((C + 2 * kStep - 1) / (2 * kStep)) * 2;   // even
 
-    // Of the 32 x 32 products of an instruction lane (g, r) gets those of a's
-    // row r with w's rows 8 i + 4 g + c (i, c = 0 .. 3) of the operand; w's row
-    // 16 g + 4 i + c is put there, so that a lane's 16 outputs are consecutive.
-    const int wrow = ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
-
+    // Lane (g, r) is lane 32 g + r.  Its addresses are computed for each tile
+    // from an opaque lane number: kept over a tile's epilogue they would be
+    // spilled, and the loop would wait for their reloads, and with them for all
+    // loads issued before, in every step.
+    //
     // Loads: one instruction brings 8 rows of 128 bytes, lane l the 16 bytes
     // that belong at position l % 8 of row l / 8.  A row's 16-byte pieces are
-    // permuted by an exclusive or with a key of the row, see `frag`.
-    const int lrow = wave * 8 + (lane >> 3), lpos = lane & 7;
-    const int akey = ((lane >> 4) & 3) | ((wave & 1) << 2);
-    const int wkey = ((lane >> 4) & 1) | ((wave >> 1) << 1) | ((lane >> 5) << 2);
-    const uint32_t acol = (uint32_t)(lpos ^ akey) * 16, wcol = (uint32_t)(lpos ^ wkey) * 16;
-    const uint32_t lbase = (uint32_t)lrow * row_bytes;
+    // permuted by an exclusive or with a key of the row.
+    //
+    // Fragments: of each group of 32 rows lane (g, r) takes the pieces g, 2 + g,
+    // 4 + g and 6 + g of one, two for each of two products.  Of the 32 x 32
+    // products of an instruction it gets those of a's row r with w's rows
+    // 8 i + 4 g + c (i, c = 0 .. 3) of the operand; w's row 16 g + 4 i + c is put
+    // there, so that a lane's 16 outputs are consecutive.
+    uint32_t acol, wcol, lbase, abase[4], wbase[2][4];
+    auto aim = [&]() {
+        const uint32_t l = opaque_v((uint32_t)lane), r = l & 31, g = l >> 5;
+        acol = ((l & 7) ^ (((l >> 4) & 3) | ((wave & 1) << 2))) * 16;
+        wcol = ((l & 7) ^ (((l >> 4) & 1) | ((wave >> 1) << 1) | ((l >> 5) << 2))) * 16;
+        lbase = (wave * 8 + (l >> 3)) * row_bytes;
+        const uint32_t wrow = ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
+        #pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t piece = ((2 * q + g) ^ ((r >> 1) & 7)) * 16;
+            abase[q] = opaque_v((wm * 64 + r) * 128 + piece);
+            wbase[0][q] = opaque_v((wn * 64 + wrow) * 128 + piece);
+            wbase[1][q] = GY == 2 ? wbase[0][q] : opaque_v((wn * 32 + wrow) * 128 + piece);
+        }
+    };
 
     struct Src { Rsrc a, w0, w1; int64_t m0, n0; } cur, nxt;
     auto source = [&](int t) {
@@ -701,14 +724,14 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         int tm, tn;
         map.place(t, tm, tn);
         s.m0 = (int64_t)tm * kTile;
-        s.n0 = (int64_t)tn * (GATED ? kHalf : kTile);
+        s.n0 = (int64_t)tn * (GATED ? kHalf : kWide);
         auto rows = [&](int64_t have, int most) {
             return (uint32_t)(have < 0 ? 0 : have < most ? have : most) * row_bytes;
         };
         s.a = rsrc(a + s.m0 * C, rows(M - s.m0, kTile));
         s.w0 = rsrc(w + s.n0 * C, rows(N - s.n0, kHalf));
         const int64_t second = GATED ? N + s.n0 : s.n0 + kHalf;
-        const uint32_t bytes1 = rows(GATED ? N - s.n0 : N - second, kHalf);
+        const uint32_t bytes1 = rows(GATED ? N - s.n0 : N - second, 64 * GY);
         s.w1 = rsrc(bytes1 ? w + second * C : w, bytes1);
         return s;
     };
@@ -727,23 +750,13 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
                  (c < row_bytes ? lbase + c : kOut) + (uint32_t)j * 32 * row_bytes);
     };
 
-    // Fragments: of each group of 32 rows lane (g, r) takes the 16-byte pieces
-    // g, 2 + g, 4 + g and 6 + g of one, two for each of two products.
-    const int key = (r >> 1) & 7;
-    uint32_t abase[4], wbase[4];
-    #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        const uint32_t piece = (uint32_t)((2 * q + g) ^ key) * 16;
-        abase[q] = opaque_v((wm * 64 + r) * 128 + piece);
-        wbase[q] = opaque_v((wn * 64 + wrow) * 128 + piece);
-    }
-    v8i fa[4][2], fw[4][2];     // [2 h + group of 32 rows][product]: half h
-    v16f acc[4][4];
+    v8i fa[4][2], fw[2 + GY][2];     // [2 h + group of 32 rows][product]: half h
+    v16f acc[4][2 + GY];
     auto zero = [&]() {
         #pragma unroll
         for (int i = 0; i < 4; i++)
             #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 2 + GY; j++)
                 #pragma unroll
                 for (int c = 0; c < 16; c++) acc[i][j][c] = 0.0f;
     };
@@ -756,17 +769,23 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
         set(fa[2 * h + s / 4][s % 4 / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 4 * 4096 + abase[s % 4]));
     };
     auto read_w = [&](int h, const uint8_t* unit, int s) {
-        set(fw[2 * h + s / 4][s % 4 / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 4 * 4096 + wbase[s % 4]));
+        set(fw[2 * h + s / 4][s % 4 / 2], s % 2, *reinterpret_cast<const v4u*>(unit + s / 4 * 4096 + wbase[h][s % 4]));
     };
-    // The 8 products of halves HA and HW, each with what `with` issues before
-    // it (LDS reads for the next phase, loads).
-    auto multiply = [&](auto HA, auto HW, auto&& with) {
+    // The products of halves HA and HW, with `reads` LDS reads for the next phase
+    // and `loads` loads spread over them.
+    auto multiply = [&](auto HA, auto HW, auto READS, auto&& read, auto LOADS, auto&& load) {
         constexpr int ha = decltype(HA)::value, hw = decltype(HW)::value;
+        constexpr int ng = hw ? GY : 2, n = 4 * ng;   // groups of w, products
+        constexpr int reads = decltype(READS)::value, loads = decltype(LOADS)::value;
         #pragma unroll
-        for (int s = 0; s < 8; s++) {
-            with(s);
-            v16f& c = acc[2 * ha + s % 4 / 2][2 * hw + s % 2];
-            c = mfma(fw[2 * hw + s % 2][s / 4], fa[2 * ha + s % 4 / 2][s / 4], c);
+        for (int s = 0; s < n; s++) {
+            #pragma unroll
+            for (int o = s * reads / n; o < (s + 1) * reads / n; o++) read(o);
+            #pragma unroll
+            for (int o = s * loads / n; o < (s + 1) * loads / n; o++) load(o);
+            const int kh = s / (2 * ng), i = s / ng % 2, f = s % ng;
+            v16f& c = acc[2 * ha + i][2 * hw + f];
+            c = mfma(fw[2 * hw + f][kh], fa[2 * ha + i][kh], c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -781,47 +800,42 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     auto step = [&](auto X, auto Y, uint8_t* a0, uint8_t* a1, uint8_t* x, uint8_t* y, uint8_t* a0n,
                     uint8_t* yn, const Src& s2, int k2) {
         constexpr int hx = decltype(X)::value, hy = decltype(Y)::value;
-        arrive<16>();
-        multiply(I0, X, [&](int s) {
-            read_w(hy, y, s);
-            if (s % 2) fetch_a(s2, k2, 0, a0, s / 2);
-        });
-        multiply(I0, Y, [&](int s) {
-            read_a(1, a1, s);
-            if (s % 2) fetch_w(s2, k2, hx, x, s / 2);
-        });
-        arrive<16>();
-        multiply(I1, Y, [&](int s) {
-            read_a(0, a0n, s);
-            if (s % 2) fetch_w(s2, k2, hy, y, s / 2);
-        });
-        multiply(I1, X, [&](int s) {
-            read_w(hy, yn, s);
-            if (s % 2) fetch_a(s2, k2, 1, a1, s / 2);
-        });
+        constexpr int wx = hx ? kW1 : kW0, wy = hy ? kW1 : kW0;
+        arrive<8 + kW0 + kW1>();         // (all but the two half steps' before)
+        multiply(I0, X, kInt<2 * wy>, [&](int s) { read_w(hy, y, s); },
+                 kInt<4>, [&](int j) { fetch_a(s2, k2, 0, a0, j); });
+        multiply(I0, Y, kInt<8>, [&](int s) { read_a(1, a1, s); },
+                 kInt<wx>, [&](int j) { fetch_w(s2, k2, hx, x, j); });
+        arrive<8 + 2 * wx>();
+        multiply(I1, Y, kInt<8>, [&](int s) { read_a(0, a0n, s); },
+                 kInt<wy>, [&](int j) { fetch_w(s2, k2, hy, y, j); });
+        multiply(I1, X, kInt<2 * wy>, [&](int s) { read_w(hy, yn, s); },
+                 kInt<4>, [&](int j) { fetch_a(s2, k2, 1, a1, j); });
     };
 
     int i = 0;
     int t = map.at(0, blockIdx.x, gridDim.x);
     if (t < 0) return;
     cur = source(t);
-    auto fetch = [&](auto&& load) {
+    aim();
+    auto fetch = [](auto LOADS, auto&& load) {
         #pragma unroll
-        for (int j = 0; j < 4; j++) load(j);
+        for (int j = 0; j < decltype(LOADS)::value; j++) load(j);
     };
     // in the order in which they are read
-    fetch([&](int j) { fetch_a(cur, 0, 0, sa00, j); });
-    fetch([&](int j) { fetch_w(cur, 0, 0, sw00, j); });
-    fetch([&](int j) { fetch_w(cur, 0, 1, sw10, j); });
-    fetch([&](int j) { fetch_a(cur, 0, 1, sa10, j); });
-    fetch([&](int j) { fetch_a(cur, 1, 0, sa01, j); });
-    fetch([&](int j) { fetch_w(cur, 1, 1, sw11, j); });
-    fetch([&](int j) { fetch_w(cur, 1, 0, sw01, j); });
-    fetch([&](int j) { fetch_a(cur, 1, 1, sa11, j); });
-    arrive<24>();
+    fetch(kInt<4>, [&](int j) { fetch_a(cur, 0, 0, sa00, j); });
+    fetch(kInt<kW0>, [&](int j) { fetch_w(cur, 0, 0, sw00, j); });
+    fetch(kInt<kW1>, [&](int j) { fetch_w(cur, 0, 1, sw10, j); });
+    fetch(kInt<4>, [&](int j) { fetch_a(cur, 0, 1, sa10, j); });
+    fetch(kInt<4>, [&](int j) { fetch_a(cur, 1, 0, sa01, j); });
+    fetch(kInt<kW1>, [&](int j) { fetch_w(cur, 1, 1, sw11, j); });
+    fetch(kInt<kW0>, [&](int j) { fetch_w(cur, 1, 0, sw01, j); });
+    fetch(kInt<4>, [&](int j) { fetch_a(cur, 1, 1, sa11, j); });
+    arrive<16 + 2 * kW1>();
     while (true) {
         const int t_next = map.at(++i, blockIdx.x, gridDim.x);
         nxt = source(t_next);
+        if (i > 1) aim();
         // (the last step of a tile before has read these pieces too, but not
         // kept them over the epilogue)
         #pragma unroll
@@ -851,36 +865,37 @@ __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
             const int64_t m = first + i * 32 + er;
             sm[i] = e.a_scale ? e.a_scale[m < M ? m : M - 1] : 1.0f;
         }
+        wait_loads<0>();   // (left to the compiler, some are waited for in the loop)
         // part: w's half, or gated the first or second 32 of the wave's outputs
-        auto finish = [&](auto PART, auto WHOLE) {
+        auto finish = [&](auto PART) {
             constexpr int part = decltype(PART)::value;
-            constexpr bool whole = decltype(WHOLE)::value;
-            const int64_t c0 = cur.n0 + wn * 64 + part * (GATED ? 32 : kHalf);
-            Residual<(GATED ? 32 : 64), 32> res[4];
-            if (e.residual) {
-                #pragma unroll
-                for (int i = 0; i < 4; i++) res[i].template load<whole>(e, ln, first + i * 32, M, c0, N);
-            }
-            Columns<GATED, 64> cols;
-            cols.template load<whole>(e, ln, c0, N);
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                #pragma unroll
-                for (int f = 0; f < 2; f++)
+            constexpr int ng = part ? GY : 2, W = GATED ? 64 : 32 * ng, CW = GATED ? 32 : W;
+            const int64_t c0 = cur.n0 + (GATED ? wn * 64 + part * 32 : part * kHalf + wn * W);
+            auto with = [&](auto WHOLE) {
+                constexpr bool whole = decltype(WHOLE)::value;
+                Residual<CW, 32> res[4];
+                if (e.residual) {
                     #pragma unroll
-                    for (int b = 0; b < 4; b++)
-                        *reinterpret_cast<v4f*>(stage + staged<64>(er, f * 8 + eg * 4 + b)) =
-                            quad(acc[i][GATED ? 2 * f + part : 2 * part + f], b, sm[i]);
-                store_staged<GATED, ACT, 64, 32, whole>(stage, e, cols, res[i], ln, first + i * 32, M, c0, N);
-            }
+                    for (int i = 0; i < 4; i++) res[i].template load<whole>(e, ln, first + i * 32, M, c0, N);
+                }
+                Columns<GATED, W> cols;
+                cols.template load<whole>(e, ln, c0, N);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    #pragma unroll
+                    for (int f = 0; f < W / 32; f++)
+                        #pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            *reinterpret_cast<v4f*>(stage + staged<W>(er, f * 8 + eg * 4 + b)) =
+                                quad(acc[i][GATED ? 2 * f + part : 2 * part + f], b, sm[i]);
+                    store_staged<GATED, ACT, W, 32, whole>(stage, e, cols, res[i], ln, first + i * 32, M, c0, N);
+                }
+            };
+            if (first + 128 <= M && c0 + CW <= N) with(std::true_type{});
+            else with(std::false_type{});
         };
-        if (first + 128 <= M && cur.n0 + (GATED ? 0 : kHalf) + wn * 64 + 64 <= N) {
-            finish(I0, std::true_type{});
-            finish(I1, std::true_type{});
-        } else {
-            finish(I0, std::false_type{});
-            finish(I1, std::false_type{});
-        }
+        finish(I0);
+        finish(I1);
         if (t_next < 0) break;
         t = t_next;
         cur = nxt;
@@ -898,9 +913,6 @@ void for_kind(bool gated, int act, F&& f) {
     };
     if (gated) with(std::true_type{}); else with(std::false_type{});
 }
-
-template <int V>
-constexpr std::integral_constant<int, V> kInt{};
 
 }  // namespace
 
@@ -1003,7 +1015,14 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
                 return;
             }
             const TileMap map = {(int)p.tiles_m, (int)p.tiles_n};
-            out = launch(linear_tile_kernel<g, ac>, std::min<int64_t>(p.tiles_m * p.tiles_n, cus), 256, a8, w8, M, N, C, map, e);
+            const int64_t blocks = std::min<int64_t>(p.tiles_m * p.tiles_n, cus);
+            if constexpr (!g) {
+                if (p.nw == 6) {
+                    out = launch(linear_tile_kernel<g, ac, 1>, blocks, 256, a8, w8, M, N, C, map, e);
+                    return;
+                }
+            }
+            out = launch(linear_tile_kernel<g, ac, 2>, blocks, 256, a8, w8, M, N, C, map, e);
         }
     });
     return out;

@@ -27,7 +27,9 @@ VARIANTS = [
     (2202, 271, 8832, False), (2752, 270, 8000, True), (535, 6809, 272, False),
     (290, 10986, 288, True), (68, 10894, 5456, False), (155, 5432, 6048, True),
     (2086, 2001, 16, False), (1665, 2436, 16, True), (137, 6258, 9568, False),
-    (67, 17438, 5872, True), (1576, 7625, 672, False), (1060, 11000, 656, True)]
+    (67, 17438, 5872, True), (1576, 7625, 672, False), (1060, 11000, 656, True),
+    (1500, 5120, 2576, False), (1801, 4099, 1040, False), (1537, 5115, 3216, False),
+    (2500, 6160, 1296, False)]
 
 
 @pytest.mark.parametrize("M,R_,C,gated", VARIANTS)

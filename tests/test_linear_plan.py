@@ -64,7 +64,9 @@ def test_tiles_cover_and_no_split_is_empty(plan, cus):
         if p["kind"] == STREAM:
             assert M <= 32 and p["bytes"] == 0
             continue
-        rows_m, rows_w = (256, 256) if p["kind"] == TILES else (32 * p["mi"], 32 * p["nw"])
+        rows_m, rows_w = 32 * p["mi"], 32 * p["nw"]
+        assert p["kind"] == MID or (rows_m, rows_w) in ((256, 256), (256, 192))
+        assert not (gated and rows_w == 192 and p["kind"] == TILES)
         assert (p["tiles_m"] - 1) * rows_m < M <= p["tiles_m"] * rows_m
         assert (p["tiles_n"] - 1) * rows_w < N * halves and p["tiles_n"] * rows_w >= N * halves
         assert 1 <= p["splits"] <= max(1, steps // 3)
@@ -80,9 +82,9 @@ def test_every_variant_is_some_products_choice(plan):
     for M, N, C, gated in _products(6000, 5):
         p = plan(M, N, C, gated)
         seen.add(("stream", p["few"]) if p["kind"] == STREAM else
-                 ("tiles",) if p["kind"] == TILES else ("mid", p["mi"], p["nw"]))
+                 ("tiles", p["nw"]) if p["kind"] == TILES else ("mid", p["mi"], p["nw"]))
     mids = {("mid", *t) for t in plan.mids()}
-    assert seen == mids | {("stream", 0), ("stream", 1), ("tiles",)}
+    assert seen == mids | {("stream", 0), ("stream", 1), ("tiles", 8), ("tiles", 6)}
 
 
 def test_few_rows_stream_the_weights(plan):
