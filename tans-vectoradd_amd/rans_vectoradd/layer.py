@@ -93,8 +93,8 @@ def fp8_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
             _explain("residual", residual, _BF16, dev)
             _require(False, "residual must have the shape of x")
         h = torch.empty_like(x)
-    q = torch.empty(shape, dtype=_U8, device=dev)
-    scale = torch.empty(shape[:-1], dtype=_F32, device=dev)
+    q = torch.empty_like(x, dtype=_U8)
+    scale = torch.empty(M if len(shape) == 2 else (), dtype=_F32, device=dev)
     _call(dev, "fp8_rmsnorm", lib.tans_fp8_rmsnorm, x.data_ptr(),
           None if residual is None else residual.data_ptr(), weight.data_ptr(), M, D, eps,
           q.data_ptr(), scale.data_ptr(), h.data_ptr())
@@ -106,9 +106,9 @@ def fp8_quantize_rows(x: torch.Tensor):
     [M] or []): scale = max(max |x| of the row, 2^-100) / 448, q =
     E4M3FN(x / scale).  D a multiple of 16."""
     M, D = _rows("x", x, _BF16)
-    dev, shape = x.device, x.shape
-    q = torch.empty(shape, dtype=_U8, device=dev)
-    scale = torch.empty(shape[:-1], dtype=_F32, device=dev)
+    dev = x.device
+    q = torch.empty_like(x, dtype=_U8)
+    scale = torch.empty(M if x.dim() == 2 else (), dtype=_F32, device=dev)
     _call(dev, "fp8_quantize_rows", lib.tans_fp8_quantize_rows, x.data_ptr(), M, D, q.data_ptr(),
           scale.data_ptr())
     return q, scale
@@ -176,7 +176,7 @@ def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor | None, w: torch.Tensor,
             _explain("residual", residual, _BF16, dev)
             _require(False, f"residual must be {list(shape)}")
         res = residual.data_ptr()
-    y = torch.empty(shape, dtype=_BF16, device=dev)
+    y = torch.empty(*shape, dtype=_BF16, device=dev)
     need = _workspace(M, R, C, bool(gated), dev.index)
     ws = torch.empty(need, dtype=_U8, device=dev) if need else None
     _call(dev, "fp8_linear", lib.tans_fp8_linear, a.data_ptr(), sa, w.data_ptr(), sw, scale, b, res,
