@@ -242,6 +242,7 @@ __global__ __launch_bounds__(KW * kLanes) void linear_stream_kernel(
         for (int j = 0; j < NF; j++)
             #pragma unroll
             for (int c = 0; c < 4; c++) part[wave][(i * NF + j) * 4 + c][lane] = acc[i][j][c];
+    wait_loads<0>();   // (loads past the last step still write into the ring)
     __syncthreads();
     // one output a thread, consecutive ones along a row of y
     const int n_rows = (int)M;
@@ -433,7 +434,6 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
     MidMap map, Epilogue e) {
     constexpr int kLoadsA = (4 * MI + NW - 1) / NW;   // of 8 rows; the last ones may be past a's
     constexpr int kA = kLoadsA * NW * 1024, kW = NW * 32 * kStep;
-    constexpr int kOut16 = GATED ? 8 : 16;      // consecutive outputs of a lane and group
     constexpr int kLoads = kLoadsA + 4;         // of a wave and step
     __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW],
         slot2[PIPE > 2 ? kA + kW : 1], slot3[PIPE > 3 ? kA + kW : 1];
