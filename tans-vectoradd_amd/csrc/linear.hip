@@ -5,8 +5,18 @@
 //   y[m][n] = act(v[m][n]) + residual[m][n]
 //   gated: y[m][j] = act(v[m][j]) * v[m][F + j] + residual[m][j], F = R / 2
 //
-// a and w hold E4M3FN bytes; the products of v_mfma_f32_16x16x128_f8f6f4 are
-// exact and summed in 32 bits; y is rounded once, to bf16.
+// a and w hold E4M3FN bytes, whose products are exact.  The matrix instructions
+// (v_mfma_f32_16x16x128_f8f6f4 and 32x32x64) add them in groups of 8 columns,
+// each product cut off at 2^-13 of its group's largest, and the groups in 32
+// bits; measured with sums that cancel, and alike for every FP8 form of the
+// instruction, so this is not a choice made here.  Everything after the sum is
+// 32-bit; the one rounding to fewer bits is y's to bf16, the type in which a
+// model keeps what lies between its layers.
+//
+// Three kernels, by what bounds them: few rows of a stream w past them (the
+// memory's rate), some rows share tiles of w (the rate at which tiles reach
+// LDS), many rows are a matrix product (the matrix cores at the board's power
+// limit).  linear_plan.h chooses.
 #include <math.h>
 
 #include <algorithm>
@@ -56,9 +66,9 @@ enum Act { kClip, kSigmoid, kErf };
 template <int ACT>
 __device__ __forceinline__ float activate(float v, const Epilogue& e) {
     if constexpr (ACT == kClip) {
-        return v < e.lo ? e.lo : v;
+        return __builtin_elementwise_maximum(v, e.lo);
     } else if constexpr (ACT == kSigmoid) {
-        // the square is kept finite, for b3 = 0 times it
+        // (the square is kept finite, for b3 = 0 times it)
         const float sq = __builtin_fminf(v * v, 1e30f);
         const float x = v * __builtin_fmaf(e.c3, sq, e.c1);
         return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x));
@@ -144,6 +154,14 @@ __device__ __forceinline__ void columns(const Epilogue& e, int64_t first, int64_
 // Few rows of a: w streamed from memory to registers.
 // ---------------------------------------------------------------------
 
+// Bound by w's bytes, read once: 34816 x 5120 (178 MB) by one row 28.7 .. 30.3 us,
+// 5.9 .. 6.2 TB/s, by 8 rows 31; 5120 x 17408 (89 MB) by one row 17.1, by 7 18
+// (4.9 .. 5.2 TB/s, of which some 3 us are the first loads' latency and the
+// join).  w loaded to registers instead of LDS, as the operands need it, takes
+// 16 bytes of 16 rows an instruction, and half of a cache line each: 42 us for
+// one row by 34816 x 5120.  With LDS, 2 waves and a pipeline of 4 steps, or 4
+// waves and 2, are within 3%; one wave a workgroup takes 47 us by 5120 x 17408.
+//
 // Products of up to 8 MA rows of a.  A workgroup takes 16 NF rows of w (gated:
 // NF / 2 groups of 16 gate rows and the value rows that belong to them); its KW
 // waves share the columns, wave k steps k, k + KW, ... of 128.  Each wave streams
@@ -424,10 +442,21 @@ struct MidMap {
 };
 
 // Workgroup: NW waves, each 32 rows of w (gated: 16 gate and 16 value rows) times
-// 32 MI rows of a; `splits` workgroups share a
-// tile's columns and leave 32-bit partial sums.  Each wave loads its own rows of
-// w and its part of a's, PIPE - 1 steps of 128 columns ahead; one barrier a
-// step.  Pieces, keys and banks as in linear_tile_kernel below.
+// 32 MI rows of a; `splits` workgroups share a tile's columns and leave 32-bit
+// partial sums.  Each wave loads its own rows of w and its part of a's, PIPE - 1
+// steps of 128 columns ahead; one barrier a step.  Pieces, keys and banks as in
+// linear_tile_kernel below.
+//
+// A step of 128 columns takes a workgroup 0.3 us (32 x 64 rows) to 1.2 (128 x
+// 256): its bytes reach LDS at 40 .. 46 GB/s a CU while all CUs load (11 TB/s
+// together), which takes longer than its products, so the best tile is the one
+// that covers the product in the fewest bytes a CU: 97 rows by 34816 x 5120 (gated)
+// 40.6 us with 128 x 160 (one round of 218 workgroups), 43.1 with 128 x 192,
+// 61.8 with 128 x 128 (two rounds), 62.4 with 64 x 128.  w is not kept in the
+// caches (non-temporal) for tiles of several rows of a: its tiles run at the
+// same time on one XCD and share it while it passes.  A product of few tiles is
+// split along its columns: 64 rows by 5120 x 17408 24.9 us in 3 parts and 37.0
+// whole, 160 by 460 x 14672 14.1 in 6 parts and 41.2.
 template <bool GATED, int ACT, int MI, int NW, int PIPE>
 __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
@@ -595,8 +624,9 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
     else finish(std::false_type{});
 }
 
-// y from the splits' sums, added in their order.  A thread takes 4 consecutive
-// outputs.
+// y from the splits' sums, added in their order (no atomics: every call gives
+// the same bits).  A thread takes 4 consecutive outputs.  Bound by its launch:
+// 2.9 us beside the sums' bytes, which lie in the caches.
 template <bool GATED, int ACT>
 __global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M, int64_t N, Epilogue e) {
     const int64_t quads = map.Np / 4;
@@ -626,6 +656,22 @@ __global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M,
 
 // ---------------------------------------------------------------------
 // Tiles of 256 rows of a by 256 rows of w, for products with many rows.
+//
+// Four waves of 128 x 128 outputs, 256 sums a lane, the most that the registers
+// hold: a step of 128 columns brings 64 KiB to LDS for 64 products of 32 x 32 x
+// 64 a wave.  8 waves of 64 x 128, or 16 x 16 x 128 products, read more of LDS
+// per product (8192^3 425 us with the latter, whose sums the compiler also moves
+// between registers in the loop).  Two steps lie in LDS, in units that are
+// refilled as soon as they are read; loads and LDS reads are spread over the
+// products (8192^3 467 us before, 431 after that).  A step takes 2230 cycles,
+// 2048 of them in the matrix cores (92%).  The workgroups are persistent, so that
+// the next tile's first steps load during the epilogue.
+//
+// 8192^3 takes 369 us, 2.98 PFLOP/s; 8192 by 34816 x 5120 (gated) 1104, 2.65; 2048 by
+// 5120 x 17408 150, 2.43.  Bound by the board's power: the clock falls to 1.65 ..
+// 1.75 GHz of 2.4 within the loop.  Besides, a tile's epilogue takes 20,000 cycles
+// in which nothing is multiplied: 17 tiles a CU by 34816 x 5120, some 15% of the
+// time, most of it the issue of 30 vector instructions an output.
 // ---------------------------------------------------------------------
 constexpr int kTile = 256;          // rows of either operand
 constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
@@ -663,7 +709,8 @@ struct TileMap {
 };
 
 // GY: groups of 32 rows of w's second half that a wave takes (2, or 1 for tiles
-// of 192 rows of w).
+// of 192 rows of w, which fit products of few tiles better: 2048 rows by 5120 x
+// 17408 are 216 of them, one round at 145 us, or 160 of 256 rows at 158).
 template <bool GATED, int ACT, int GY>
 __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
