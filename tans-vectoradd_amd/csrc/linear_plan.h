@@ -61,6 +61,8 @@ inline Plan plan(int64_t M, int64_t N, int64_t C, bool gated, int cus) {
     float best = 0.0f;
     auto consider = [&](Kind kind, const Tile& t, int splits) {
         const int64_t tm = parts(M, 32 * t.mi), tn = parts(N, 32 * t.nw / halves);
+        // (a launch has fewer than 2^31 threads; the large tiles' stay)
+        if (kind == kMid && tm * tn * splits > INT32_MAX / (64 * t.nw)) return;
         const float rounds = (float)parts(tm * tn * splits, cus);
         float us = kLaunch + rounds * (t.round + (float)parts(steps, splits) * t.step);
         us = std::max(us, kLaunch + 1.0f + (float)w_bytes / kReadRate);

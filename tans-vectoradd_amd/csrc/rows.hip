@@ -277,14 +277,13 @@ int rows_check(const char* what, const void* x, int64_t M, int64_t D, const void
 // 73.5.  Up to some hundred rows a call takes the 4.0 .. 4.5 us of a launch at
 // either.
 template <bool NORM, bool RES>
-int rows_launch(const void* x, const void* residual, const void* weight, int64_t M, int64_t D,
-                float eps, void* q, float* scale, void* h, void* stream) {
+int rows_launch(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, int64_t M,
+                int64_t D, float eps, uint8_t* q, float* scale, uint16_t* h, hipStream_t stream) {
     const int V = (int)(D / kVec);
     if (V > kMaxVecs * kMaxWaves * kLanes) {
         hipLaunchKernelGGL((long_rows_kernel<NORM, RES>), dim3((unsigned)M),
-                           dim3(kMaxWaves * kLanes), 0, (hipStream_t)stream, (const uint16_t*)x,
-                           (const uint16_t*)residual, (const uint16_t*)weight, V, eps, (uint8_t*)q,
-                           scale, (uint16_t*)h);
+                           dim3(kMaxWaves * kLanes), 0, stream, x, residual, weight, V, eps, q,
+                           scale, h);
         return hip_check(hipGetLastError(), "long_rows_kernel launch");
     }
     const int waves1 = (V + kLanes - 1) / kLanes;   // waves at one vector a thread
@@ -295,9 +294,8 @@ int rows_launch(const void* x, const void* residual, const void* weight, int64_t
     const unsigned blocks = nw == 1 ? (unsigned)((M + solo_rows - 1) / solo_rows) : (unsigned)M;
     const unsigned threads = (nw == 1 ? solo_rows : nw) * kLanes;
     auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, (hipStream_t)stream,
-                           (const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)weight,
-                           M, V, nw, eps, (uint8_t*)q, scale, (uint16_t*)h);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, x, residual, weight, M, V,
+                           nw, eps, q, scale, h);
     };
     switch (nv) {
         case 1: launch(rows_kernel<NORM, RES, 1>); break;
@@ -309,6 +307,22 @@ int rows_launch(const void* x, const void* residual, const void* weight, int64_t
         default: launch(rows_kernel<NORM, RES, 7>); break;
     }
     return hip_check(hipGetLastError(), "rows_kernel launch");
+}
+
+// All rows, in calls of at most kCallRows: a launch has fewer than 2^32 threads.
+constexpr int64_t kCallRows = int64_t(1) << 21;   // of up to 1024 threads
+
+template <bool NORM, bool RES>
+int rows_all(const void* x, const void* residual, const void* weight, int64_t M, int64_t D,
+             float eps, void* q, float* scale, void* h, void* stream) {
+    for (int64_t m = 0; m < M; m += kCallRows) {
+        const int rc = rows_launch<NORM, RES>(
+            (const uint16_t*)x + m * D, RES ? (const uint16_t*)residual + m * D : nullptr,
+            (const uint16_t*)weight, std::min(M - m, kCallRows), D, eps, (uint8_t*)q + m * D,
+            scale + m, RES ? (uint16_t*)h + m * D : nullptr, (hipStream_t)stream);
+        if (rc != TANS_OK) return rc;
+    }
+    return TANS_OK;
 }
 
 }  // namespace
@@ -323,15 +337,15 @@ int tans_fp8_rmsnorm(const void* x, const void* residual, const void* weight, in
     if (!aligned(weight, 16) || !aligned(residual, 16) || !aligned(h, 16))
         return fail(TANS_EINVAL, "rmsnorm: misaligned buffer (rows and weight 16 bytes)");
     if (!(eps >= 0.0f)) return fail(TANS_EINVAL, "rmsnorm: eps must not be negative");
-    return residual ? rows_launch<true, true>(x, residual, weight, M, D, eps, q, scale, h, stream)
-                    : rows_launch<true, false>(x, nullptr, weight, M, D, eps, q, scale, nullptr, stream);
+    return residual ? rows_all<true, true>(x, residual, weight, M, D, eps, q, scale, h, stream)
+                    : rows_all<true, false>(x, nullptr, weight, M, D, eps, q, scale, nullptr, stream);
 }
 
 int tans_fp8_quantize_rows(const void* x, int64_t M, int64_t D, void* q, float* scale,
                            void* stream) {
     const int rc = rows_check("quantize_rows", x, M, D, q, scale);
     if (rc != TANS_OK || M == 0) return rc;
-    return rows_launch<false, false>(x, nullptr, nullptr, M, D, 0.0f, q, scale, nullptr, stream);
+    return rows_all<false, false>(x, nullptr, nullptr, M, D, 0.0f, q, scale, nullptr, stream);
 }
 
 }  // extern "C"

@@ -105,6 +105,44 @@ def test_quantize_rows_matches_64_bits(M, D):
     assert torch.equal(scale, (x.double().abs().amax(dim=1) / 448.0).float())
 
 
+# rows of 4, 6 and 7 loads a thread, and the longest that a workgroup holds
+@pytest.mark.parametrize("D", [12304, 16384, 40976, 49152, 49168, 57344, 57360])
+@pytest.mark.parametrize("op", ["norm", "norm_residual", "quantize"])
+def test_long_rows_match_64_bits(D, op):
+    import rans_vectoradd as R
+    _say(f"case: {op} 3x{D}")
+    g = _gen(D)
+    x = _bf16(g, 3, D, std=2.0)
+    if op == "quantize":
+        q, scale = R.fp8_quantize_rows(x)
+        _check_q(q, scale, x.double())
+        return
+    res = _bf16(g, 3, D) if op == "norm_residual" else None
+    w = _bf16(g, D)
+    q, scale, h = R.fp8_rmsnorm(x, w, res, eps=1e-5)
+    if res is not None:
+        assert torch.equal(h, (x.float() + res.float()).to(torch.bfloat16))
+    _check_q(q, scale, _norm64(x, w, res, 1e-5))
+
+
+def test_more_rows_than_one_launch_has_threads_for():
+    import rans_vectoradd as R
+    n, times = 1024, (1 << 16) + 1          # 2^26 + 1024 rows of one wave each
+    _say(f"case: quantize_rows and rmsnorm of {n * times} rows")
+    g = _gen(5)
+    x, res, w = _bf16(g, n, 16), _bf16(g, n, 16), _bf16(g, 16)
+    many = x.repeat(times, 1)
+    q0, s0 = R.fp8_quantize_rows(x)
+    q, s = R.fp8_quantize_rows(many)
+    assert torch.equal(q.view(times, n, 16), q0.expand(times, n, 16))
+    assert torch.equal(s.view(times, n), s0.expand(times, n))
+    q0, s0, h0 = R.fp8_rmsnorm(x, w, res)
+    q, s, h = R.fp8_rmsnorm(many, w, res.repeat(times, 1))
+    assert torch.equal(q.view(times, n, 16), q0.expand(times, n, 16))
+    assert torch.equal(s.view(times, n), s0.expand(times, n))
+    assert torch.equal(h.view(torch.int16).view(times, n, 16), h0.view(torch.int16).expand(times, n, 16))
+
+
 def test_rows_of_zeros_and_tiny_and_huge_values():
     import rans_vectoradd as R
     D = 272

@@ -93,3 +93,13 @@ def test_few_rows_stream_the_weights(plan):
     assert plan(24, 3403, 5232, True)["kind"] == STREAM     # w of 36 MB
     assert plan(24, 17408, 5120, True)["kind"] == MID       # of 178 MB
     assert plan(1, 4096, 4096, False)["few"] and not plan(1, 7000, 4096, False)["few"]
+
+
+def test_launches_stay_below_2_31_threads(plan):
+    for M, N, C, gated in ((2 ** 31 - 1, 16, 16, False), (2 ** 31 - 1, 16, 16, True),
+                           (2 ** 28, 300, 2048, False), (17, 2 ** 27, 16, False), (100, 2 ** 26, 16, True)):
+        p = plan(M, N, C, gated)
+        if p["kind"] == MID:
+            assert p["tiles_m"] * p["tiles_n"] * p["splits"] * 64 * p["nw"] < 2 ** 31
+        elif p["kind"] == TILES:
+            assert p["tiles_m"] * p["tiles_n"] < 2 ** 31
