@@ -452,7 +452,8 @@ struct MidMap {
 // together), which takes longer than its products, so the best tile is the one
 // that covers the product in the fewest bytes a CU: 97 rows by 34816 x 5120 (gated)
 // 40.6 us with 128 x 160 (one round of 218 workgroups), 43.1 with 128 x 192,
-// 61.8 with 128 x 128 (two rounds), 62.4 with 64 x 128.  w is not kept in the
+// 61.8 with 128 x 128 (two rounds), 62.4 with 64 x 128; 192 rows 52.4 with 192 x
+// 160, 68.0 with 256 x 256 on half of the CUs.  w is not kept in the
 // caches (non-temporal) for tiles of several rows of a: its tiles run at the
 // same time on one XCD and share it while it passes.  A product of few tiles is
 // split along its columns: 64 rows by 5120 x 17408 24.9 us in 3 parts and 37.0
@@ -464,8 +465,9 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
     constexpr int kLoadsA = (4 * MI + NW - 1) / NW;   // of 8 rows; the last ones may be past a's
     constexpr int kA = kLoadsA * NW * 1024, kW = NW * 32 * kStep;
     constexpr int kLoads = kLoadsA + 4;         // of a wave and step
-    __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW],
-        slot2[PIPE > 2 ? kA + kW : 1], slot3[PIPE > 3 ? kA + kW : 1];
+    static_assert(PIPE == 3 || PIPE == 4, "slots");
+    __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW], slot2[kA + kW],
+        slot3[PIPE > 3 ? kA + kW : 1];
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int r = lane & 31, g = lane >> 5;
@@ -551,14 +553,11 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
         }
     };
     fetch(0, slot0);
-    if (PIPE > 2) fetch(1, slot1);
+    fetch(1, slot1);
     if (PIPE > 3) fetch(2, slot2);
     // (steps past the split's last are zeros)
     for (int k = 0; k < k_end - k_first; k += PIPE) {
-        if constexpr (PIPE == 2) {
-            step(k, slot0, slot1);
-            step(k + 1, slot1, slot0);
-        } else if constexpr (PIPE == 3) {
+        if constexpr (PIPE == 3) {
             step(k, slot0, slot2);
             step(k + 1, slot1, slot0);
             step(k + 2, slot2, slot1);
@@ -1054,6 +1053,7 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
             mid(kInt<4>, kInt<5>);
             mid(kInt<4>, kInt<6>);
             mid(kInt<4>, kInt<8>);
+            mid(kInt<6>, kInt<5>);
             if (out == TANS_OK && p.splits > 1)
                 out = launch(linear_join_kernel<g, ac>, (M * (p.Np / 4) + 255) / 256, 256, map, M, N, e);
         } else {

@@ -31,11 +31,14 @@ struct Tile { int mi, nw; float step, round; };
 constexpr Tile kMids[] = {
     {1, 2, 0.29f, 0.4f}, {1, 4, 0.50f, 0.2f}, {2, 4, 0.56f, 1.4f}, {2, 5, 0.70f, 1.7f},
     {3, 4, 0.65f, 2.0f}, {4, 4, 0.72f, 3.0f}, {4, 5, 0.88f, 3.7f}, {4, 6, 0.97f, 2.8f},
-    {4, 8, 1.21f, 2.2f}};
+    {4, 8, 1.21f, 2.2f}, {6, 5, 1.22f, 4.3f}};
 // The large tiles: 256 rows of a by 256, or not gated 192, rows of w.  Down
 // 5120 x 17408: 2048 rows of a 158 / 145 us, 4096 334 / 290; 3000 by 5120 x
 // 5120 68 / 91, 1500 52 / 45.
-constexpr Tile kBig = {8, 8, 1.15f, 12.0f}, kBig192 = {8, 6, 1.05f, 4.0f};
+// A gated tile's epilogue takes longer (512 rows by 34816 x 5120: two rounds of
+// these 132 us, three of 128 x 192 118).
+constexpr Tile kBig = {8, 8, 1.15f, 12.0f}, kBigGated = {8, 8, 1.15f, 18.0f},
+               kBig192 = {8, 6, 1.05f, 4.0f};
 constexpr float kLaunch = 4.0f, kJoin = 2.9f;        // us: a call; the second kernel
 constexpr float kReadRate = 5.9e6f;                  // bytes of w a us
 constexpr float kSumRate = 4.6e6f;                   // bytes of partial sums a us
@@ -76,7 +79,7 @@ inline Plan plan(int64_t M, int64_t N, int64_t C, bool gated, int cus) {
         p.tiles_m = tm;
         p.tiles_n = tn;
     };
-    consider(kTiles, kBig, 1);
+    consider(kTiles, gated ? kBigGated : kBig, 1);
     if (!gated) consider(kTiles, kBig192, 1);
     for (const Tile& t : kMids) {
         for (int s = 1; s <= kMaxSplits && (s == 1 || steps >= 3 * s); s++) consider(kMid, t, s);

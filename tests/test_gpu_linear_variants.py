@@ -104,3 +104,14 @@ def test_linear_sums_that_cancel_exactly(M, C):
     w[1::2, ::2] = 0xC0                                                    # -2.0
     y = R.fp8_linear(a, None, w)
     assert (y[:, 0::2] == 2.0 * C).all() and (y[:, 1::2] == 0.0).all()
+
+
+# tiles of 192 x 160 rows and gated ones of 256 x 256
+@pytest.mark.parametrize("M,R_,C,gated", [
+    (190, 34838, 272, False), (191, 34818, 272, True), (557, 13136, 16, True),
+    (136, 17968, 6128, False), (131, 16398, 6096, True), (290, 32730, 1376, True),
+    (643, 17400, 656, False)])
+def test_linear_wide_tiles(M, R_, C, gated):
+    L._say(f"case: linear {M}x{R_}x{C} gated={gated}")
+    L._run_linear(M, R_, C, "silu" if gated else "none", gated, bias=True, residual=True)
+    L._run_linear(M, R_, C, "gelu", gated, seed=1)
