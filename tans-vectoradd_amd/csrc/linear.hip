@@ -52,25 +52,25 @@ struct Epilogue {
     uint16_t* y;                 // bf16 [M, N]
     float scale;
     float lo;                    // kClip: the least value
-    float c1, c3;                // kSigmoid: of the sigmoid's argument, times log2 e
 };
 
-// The activations in three forms, each a kernel of its own:
-//   kClip     max(v, lo): none (lo = -infinity) and ReLU (a NaN stays one)
-//   kSigmoid  v * sigmoid(b1 v + b3 v^3): SiLU (b1 = 1, b3 = 0) and GELU's tanh
-//             form, (1 + tanh(u)) / 2 = sigmoid(2 u)
-//   kErf      v Phi(v), erfc by Abramowitz and Stegun 7.1.26 (absolute error
-//             below 1.5e-7)
-enum Act { kClip, kSigmoid, kErf };
+// The activations in four forms, each a kernel of its own:
+//   kClip  max(v, lo): none (lo = -infinity) and ReLU (a NaN stays one)
+//   kSilu  v sigmoid(v)
+//   kTanh  GELU's tanh form: (1 + tanh(u)) / 2 = sigmoid(2 u)
+//   kErf   v Phi(v), erfc by Abramowitz and Stegun 7.1.26 (absolute error
+//          below 1.5e-7)
+enum Act { kClip, kSilu, kTanh, kErf };
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v, const Epilogue& e) {
     if constexpr (ACT == kClip) {
         return __builtin_elementwise_maximum(v, e.lo);
-    } else if constexpr (ACT == kSigmoid) {
-        // (the square is kept finite, for b3 = 0 times it)
-        const float sq = __builtin_fminf(v * v, 1e30f);
-        const float x = v * __builtin_fmaf(e.c3, sq, e.c1);
+    } else if constexpr (ACT == kSilu) {
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
+    } else if constexpr (ACT == kTanh) {
+        constexpr float c1 = 2.0f * 0.79788456f * kLog2e;   // 2 sqrt(2 / pi), to base 2
+        const float x = v * __builtin_fmaf(0.044715f * c1, v * v, c1);
         return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x));
     } else {
         const float x = __builtin_fabsf(v) * 0.70710678f;
@@ -954,7 +954,8 @@ template <class F>
 void for_kind(bool gated, int act, F&& f) {
     auto with = [&](auto G) {
         if (act == kErf) f(G, std::integral_constant<int, kErf>{});
-        else if (act == kSigmoid) f(G, std::integral_constant<int, kSigmoid>{});
+        else if (act == kTanh) f(G, std::integral_constant<int, kTanh>{});
+        else if (act == kSilu) f(G, std::integral_constant<int, kSilu>{});
         else f(G, std::integral_constant<int, kClip>{});
     };
     if (gated) with(std::true_type{}); else with(std::false_type{});
@@ -1002,14 +1003,12 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
         return fail(TANS_EINVAL, "linear: workspace too small, null or misaligned (16 bytes)");
     const int64_t N = gated ? R / 2 : R;
     if (cus <= 0) return fail(TANS_EHIP, "linear: cannot query the device's CU count");
-    const float tanh_c1 = 2.0f * 0.79788456f * kLog2e;   // 2 sqrt(2 / pi)
-    const bool tanh_form = activation == TANS_ACT_GELU_TANH;
     const Epilogue e = {a_scale, w_scale, (const uint16_t*)bias, (const uint16_t*)residual,
                         (uint16_t*)y, scale,
-                        activation == TANS_ACT_RELU ? 0.0f : -INFINITY,
-                        tanh_form ? tanh_c1 : kLog2e, tanh_form ? 0.044715f * tanh_c1 : 0.0f};
+                        activation == TANS_ACT_RELU ? 0.0f : -INFINITY};
     const int act = activation == TANS_ACT_GELU ? kErf
-                    : activation == TANS_ACT_SILU || tanh_form ? kSigmoid : kClip;
+                    : activation == TANS_ACT_GELU_TANH ? kTanh
+                    : activation == TANS_ACT_SILU ? kSilu : kClip;
     const uint8_t *a8 = (const uint8_t*)a, *w8 = (const uint8_t*)w;
     const hipStream_t st = (hipStream_t)stream;
     auto launch = [&](auto kernel, int64_t blocks, int threads, auto... args) {
