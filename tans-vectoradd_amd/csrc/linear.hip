@@ -458,16 +458,20 @@ struct MidMap {
 // same time on one XCD and share it while it passes.  A product of few tiles is
 // split along its columns: 64 rows by 5120 x 17408 24.9 us in 3 parts and 37.0
 // whole, 160 by 460 x 14672 14.1 in 6 parts and 41.2.
+//
+// With PIPE = 2 two workgroups share a CU, and one's products hide the other's
+// loads and epilogue: for products of few steps, which are mostly those
+// (linear_plan.h has what it gains).
 template <bool GATED, int ACT, int MI, int NW, int PIPE>
-__global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
+__global__ __launch_bounds__(NW * kLanes, PIPE == 2 ? 2 : 1) void linear_mid_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,
     MidMap map, Epilogue e) {
     constexpr int kLoadsA = (4 * MI + NW - 1) / NW;   // of 8 rows; the last ones may be past a's
     constexpr int kA = kLoadsA * NW * 1024, kW = NW * 32 * kStep;
     constexpr int kLoads = kLoadsA + 4;         // of a wave and step
-    static_assert(PIPE == 3 || PIPE == 4, "slots");
-    __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW], slot2[kA + kW],
-        slot3[PIPE > 3 ? kA + kW : 1];
+    static_assert(PIPE >= 2 && PIPE <= 4, "slots");
+    __shared__ __attribute__((aligned(1024))) uint8_t slot0[kA + kW], slot1[kA + kW],
+        slot2[PIPE > 2 ? kA + kW : 1], slot3[PIPE > 3 ? kA + kW : 1];
     const int lane = threadIdx.x & (kLanes - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int r = lane & 31, g = lane >> 5;
@@ -553,11 +557,14 @@ __global__ __launch_bounds__(NW * kLanes) void linear_mid_kernel(
         }
     };
     fetch(0, slot0);
-    fetch(1, slot1);
+    if (PIPE > 2) fetch(1, slot1);
     if (PIPE > 3) fetch(2, slot2);
     // (steps past the split's last are zeros)
     for (int k = 0; k < k_end - k_first; k += PIPE) {
-        if constexpr (PIPE == 3) {
+        if constexpr (PIPE == 2) {
+            step(k, slot0, slot1);
+            step(k + 1, slot1, slot0);
+        } else if constexpr (PIPE == 3) {
             step(k, slot0, slot2);
             step(k + 1, slot1, slot0);
             step(k + 2, slot2, slot1);
@@ -1049,6 +1056,10 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
                 if (p.mi == mi && p.nw == nw)
                     out = launch(linear_mid_kernel<g, ac, mi, nw, pipe>, blocks, nw * kLanes, a8, w8, M, N, C, map, e);
             };
+            if (p.pairs) {
+                out = launch(linear_mid_kernel<g, ac, 4, 4, 2>, blocks, 4 * kLanes, a8, w8, M, N, C, map, e);
+                return;
+            }
             mid(kInt<1>, kInt<2>);
             mid(kInt<1>, kInt<4>);
             mid(kInt<2>, kInt<4>);

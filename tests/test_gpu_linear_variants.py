@@ -115,3 +115,13 @@ def test_linear_wide_tiles(M, R_, C, gated):
     L._say(f"case: linear {M}x{R_}x{C} gated={gated}")
     L._run_linear(M, R_, C, "silu" if gated else "none", gated, bias=True, residual=True)
     L._run_linear(M, R_, C, "gelu", gated, seed=1)
+
+
+# few steps and many tiles: 128 x 128, two workgroups a CU
+@pytest.mark.parametrize("M,R_,C,gated", [
+    (2049, 4099, 16, False), (2047, 4354, 144, True), (4225, 2049, 272, False),
+    (1151, 7938, 384, True), (363, 22017, 528, False), (1537, 5633, 768, False)])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "gelu_tanh"])
+def test_linear_two_workgroups_a_cu(M, R_, C, gated, act):
+    L._say(f"case: linear pairs {M}x{R_}x{C} {act} gated={gated}")
+    L._run_linear(M, R_, C, act, gated, bias=True, residual=True)
