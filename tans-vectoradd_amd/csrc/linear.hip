@@ -451,7 +451,7 @@ struct MidMap {
 // 256): its bytes reach LDS at 40 .. 46 GB/s a CU while all CUs load (11 TB/s
 // together), which takes longer than its products, so the best tile is the one
 // that covers the product in the fewest bytes a CU: 97 rows by 34816 x 5120 (gated)
-// 40.6 us with 128 x 160 (one round of 218 workgroups), 43.1 with 128 x 192,
+// 39.4 us with 128 x 160 (one round of 218 workgroups), 43.1 with 128 x 192,
 // 61.8 with 128 x 128 (two rounds), 62.4 with 64 x 128; 192 rows 52.4 with 192 x
 // 160, 68.0 with 256 x 256 on half of the CUs.  w is not kept in the
 // caches (non-temporal) for tiles of several rows of a: its tiles run at the
@@ -677,7 +677,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M,
 // 5120 x 17408 150, 2.43.  Bound by the board's power: the clock falls to 1.65 ..
 // 1.75 GHz of 2.4 within the loop.  Besides, a tile's epilogue takes 20,000 cycles
 // in which nothing is multiplied: 17 tiles a CU by 34816 x 5120, some 15% of the
-// time, most of it the issue of 30 vector instructions an output.
+// time, most of it the issue of 27 vector instructions an output.
 // ---------------------------------------------------------------------
 constexpr int kTile = 256;          // rows of either operand
 constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
