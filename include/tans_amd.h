@@ -330,8 +330,11 @@ int tans_fp8_gemm_raw(const void* w, int64_t R, int64_t C, const void* x, int64_
  *   y = h * weight / sqrt(mean(h^2) + eps)            (fp32, from unrounded h)
  *   scale[m] = max(max over the row of |y|, 2^-100) / 448
  *   q = E4M3FN(y / scale[m]), nearest even
- * A row that holds a NaN or an infinity gets NaN bytes in its place at
- * least, and a scale that is not finite; other rows are not affected.
+ * Right for any finite h and eps: rows whose squares leave the range of 32
+ * bits are scaled by a power of two first.  (Zeros with eps = 0 are 0 / 0, a
+ * NaN.)  A row whose h or y holds a NaN or, as a 32-bit value, an infinity gets
+ * NaN bytes in its place at least, and a scale that is not finite; other rows
+ * are not affected.
  *   x, residual, h  bf16 [M, D]; residual NULL: h = x, not stored (h unused).
  *                   h may be x or residual
  *   weight          bf16 [D]

@@ -10,7 +10,10 @@
 // Sums, maximum and scale are 32-bit.  h is kept as bf16 because the next layer
 // reads it as its residual; y only as 8 bits, with a scale for each row.
 //
-// h^2 is summed from the unrounded h.  The maximum is taken over the bits of
+// h^2 is summed from the unrounded h.  Where mean(h^2) + eps is outside 2^-100 ..
+// 2^128 (a 32-bit square has overflowed, or lost bits below 2^-126 that count),
+// the sum is taken again of h times a power of two, so that the norm of any
+// finite row is right.  The maximum is taken over the bits of
 // |y| as unsigned numbers, in which a NaN is larger than infinity: a row that
 // holds one, or an infinity, comes out with a scale that is not finite and
 // NaN bytes.
@@ -111,6 +114,24 @@ __device__ __forceinline__ v2u to_fp8(const float (&y)[kVec], float sc, float in
     return r;
 }
 
+// Whether mean(h^2) + eps can be trusted: sums of squares that overflow are
+// infinite, and squares below 2^-126 lose at most 2^-126 each, 2^-26 of the
+// least mean here.  Alike in all lanes that share a row, so one scalar branch.
+__device__ __forceinline__ bool in_range(float mean) {
+    constexpr uint32_t kLeast = (127 - 100) << 23, kInf = 255u << 23;
+    const uint32_t u = (uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mean));
+    return u - kLeast < kInf - kLeast;
+}
+
+// A power of two that brings a row's largest |h| to 1 .. 4, or by 2^100 at most:
+// then a square is never lost beside the row's largest, nor does eps f^2 overflow
+// where the mean was too small (eps < 2^-100).
+__device__ __forceinline__ float rescale(float top) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);   // 255 with NaN and infinity
+    const int f = 254 - e < 1 ? 1 : 254 - e > 227 ? 227 : 254 - e;
+    return __builtin_bit_cast(float, (uint32_t)f << 23);
+}
+
 template <bool NORM, bool RES>
 struct Row {
     // vector i of the row: h, and the residual's sum as it is stored
@@ -130,6 +151,10 @@ struct Row {
         #pragma unroll
         for (int k = 0; k < kVec; k++) s = __builtin_fmaf(h[k], h[k], s);
         return s;
+    }
+    static __device__ __forceinline__ void scale_by(float (&h)[kVec], float f) {
+        #pragma unroll
+        for (int k = 0; k < kVec; k++) h[k] *= f;
     }
     static __device__ __forceinline__ void normed(float (&h)[kVec], const v4u& w, float inv) {
         if constexpr (NORM) {
@@ -161,7 +186,7 @@ __global__ __launch_bounds__(kMaxWaves * kLanes) void rows_kernel(
     const uint16_t* x, const uint16_t* residual, const uint16_t* __restrict__ weight, int64_t M,
     int V, int nw, float eps, uint8_t* __restrict__ q, float* __restrict__ scale, uint16_t* h) {
     using P = Row<NORM, RES>;
-    __shared__ float part_s[kMaxWaves], part_m[kMaxWaves];
+    __shared__ float part_s[kMaxWaves], part_m[kMaxWaves], part_h[kMaxWaves], part_t[kMaxWaves];
     const bool solo = nw == 1;
     const int T = nw * kLanes;
     const int t = solo ? threadIdx.x & (kLanes - 1) : threadIdx.x;
@@ -195,7 +220,23 @@ __global__ __launch_bounds__(kMaxWaves * kLanes) void rows_kernel(
         if (NORM) s = P::squares(y[j], s);
     }
     float inv = 1.0f;
-    if (NORM) inv = 1.0f / sqrtf(row_join<Sum>(s, part_s, nw) / (float)D + eps);
+    if (NORM) {
+        float mean = row_join<Sum>(s, part_s, nw) / (float)D + eps;
+        if (!in_range(mean)) {
+            float most = 0.0f;
+            #pragma unroll
+            for (int j = 0; j < NV; j++) most = amax8(y[j], most);
+            const float f = rescale(row_join<Max>(most, part_h, nw));
+            s = 0.0f;
+            #pragma unroll
+            for (int j = 0; j < NV; j++) {
+                P::scale_by(y[j], f);
+                s = P::squares(y[j], s);
+            }
+            mean = row_join<Sum>(s, part_t, nw) / (float)D + eps * f * f;
+        }
+        inv = 1.0f / sqrtf(mean);
+    }
     float top = __builtin_bit_cast(float, kAmaxMinBits);
     #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -214,13 +255,14 @@ __global__ __launch_bounds__(kMaxWaves * kLanes) void rows_kernel(
 }
 
 // Rows longer than a workgroup holds in registers (57344 elements): three
-// passes, the second and third reading what the first left in the caches.
+// passes (five where the squares leave their range), the later ones reading what
+// the first left in the caches.
 template <bool NORM, bool RES>
 __global__ __launch_bounds__(kMaxWaves * kLanes) void long_rows_kernel(
     const uint16_t* x, const uint16_t* residual, const uint16_t* __restrict__ weight, int V,
     float eps, uint8_t* __restrict__ q, float* __restrict__ scale, uint16_t* h) {
     using P = Row<NORM, RES>;
-    __shared__ float part_s[kMaxWaves], part_m[kMaxWaves];
+    __shared__ float part_s[kMaxWaves], part_m[kMaxWaves], part_h[kMaxWaves], part_t[kMaxWaves];
     constexpr int T = kMaxWaves * kLanes;
     const int64_t row = blockIdx.x;
     const int64_t D = (int64_t)V * kVec;
@@ -228,7 +270,7 @@ __global__ __launch_bounds__(kMaxWaves * kLanes) void long_rows_kernel(
         const v4u xv = P::load(x + row * D, i);
         P::sum(xv, RES ? P::load(residual + row * D, i) : xv, f);
     };
-    float inv = 1.0f;
+    float inv = 1.0f, by = 1.0f;   // of h's power of two
     float f[kVec];
     if (NORM) {
         float s = 0.0f;
@@ -236,9 +278,28 @@ __global__ __launch_bounds__(kMaxWaves * kLanes) void long_rows_kernel(
             sum_at(i, f);
             s = P::squares(f, s);
         }
-        inv = 1.0f / sqrtf(row_join<Sum>(s, part_s, kMaxWaves) / (float)D + eps);
+        float mean = row_join<Sum>(s, part_s, kMaxWaves) / (float)D + eps;
+        if (!in_range(mean)) {
+            float most = 0.0f;
+            for (int i = threadIdx.x; i < V; i += T) {
+                sum_at(i, f);
+                most = amax8(f, most);
+            }
+            by = rescale(row_join<Max>(most, part_h, kMaxWaves));
+            s = 0.0f;
+            for (int i = threadIdx.x; i < V; i += T) {
+                sum_at(i, f);
+                P::scale_by(f, by);
+                s = P::squares(f, s);
+            }
+            mean = row_join<Sum>(s, part_t, kMaxWaves) / (float)D + eps * by * by;
+        }
+        inv = 1.0f / sqrtf(mean);
     }
-    auto y_at = [&](int i) { P::normed(f, NORM ? P::load(weight, i) : v4u{0, 0, 0, 0}, inv); };
+    auto y_at = [&](int i) {
+        if (NORM) P::scale_by(f, by);
+        P::normed(f, NORM ? P::load(weight, i) : v4u{0, 0, 0, 0}, inv);
+    };
     float top = __builtin_bit_cast(float, kAmaxMinBits);
     for (int i = threadIdx.x; i < V; i += T) {
         sum_at(i, f);

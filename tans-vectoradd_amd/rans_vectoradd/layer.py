@@ -78,8 +78,8 @@ def fp8_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
 
     x, residual: bf16 [D] or [M, D], D a multiple of 16; weight bf16 [D].
     scale = max(max |y| of the row, 2^-100) / 448 and q = E4M3FN(y / scale).
-    The norm is taken of the sum in 32 bits; h is that sum as bf16 (without
-    residual: x itself)."""
+    The norm is taken of the sum in 32 bits, of whatever finite size; h is that
+    sum as bf16 (without residual: x itself)."""
     M, D = _rows("x", x, _BF16)
     dev, shape = x.device, x.shape
     if not (_ok(weight, _BF16, dev) and weight.shape == (D,) and eps >= 0.0):
