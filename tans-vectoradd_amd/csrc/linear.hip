@@ -427,14 +427,6 @@ __device__ __forceinline__ void store_staged(const float* stage, const Epilogue&
     wave_sync();
 }
 
-// Workgroups run on XCD (block % 8): a permutation of the blocks that gives each
-// XCD a run of neighbours.
-constexpr int kXcds = 8;
-__device__ __forceinline__ int xcd_order(int block, int blocks) {
-    const int xcd = block % kXcds, per = blocks / kXcds, more = blocks % kXcds;
-    return xcd * per + (xcd < more ? xcd : more) + block / kXcds;
-}
-
 struct MidMap {
     int tiles_m, tiles_n, splits;
     int64_t Np;       // outputs of a row of partial sums, a multiple of 16
@@ -683,36 +675,6 @@ constexpr int kTile = 256;          // rows of either operand
 constexpr int kHalf = 128;          // w's rows come in two halves (gated: gate and value)
 constexpr int kUnit = kHalf * kStep;
 constexpr int kTileWaves = 4;
-
-// Where a workgroup's tiles lie: the tile sequence takes groups of kGroupM
-// tiles of a's rows, in each of them w's tiles in order and the group's row
-// tiles innermost; an eighth of the sequence goes to each of the 8 XCDs
-// (workgroup b runs on XCD b % 8), so that the tiles an XCD works on at a time
-// share their rows of a and w in its L2.
-constexpr int kGroupM = 8;
-
-struct TileMap {
-    int tiles_m, tiles_n;
-    __device__ __forceinline__ int count() const { return tiles_m * tiles_n; }
-    // the i-th tile of workgroup b of `blocks`, or -1
-    __device__ __forceinline__ int at(int i, int b, int blocks) const {
-        const int xcd = b % kXcds, T = count();
-        const int per = T / kXcds, more = T % kXcds;
-        const int first = xcd * per + (xcd < more ? xcd : more);
-        const int n = per + (xcd < more ? 1 : 0);
-        const int peers = (blocks - xcd + kXcds - 1) / kXcds;
-        const int k = i * peers + b / kXcds;
-        return k < n ? first + k : -1;
-    }
-    __device__ __forceinline__ void place(int t, int& tm, int& tn) const {
-        const int group = t / (kGroupM * tiles_n);
-        const int m_first = group * kGroupM;
-        const int gm = tiles_m - m_first < kGroupM ? tiles_m - m_first : kGroupM;
-        const int in = t - group * kGroupM * tiles_n;
-        tm = m_first + in % gm;
-        tn = in / gm;
-    }
-};
 
 // GY: groups of 32 rows of w's second half that a wave takes (2, or 1 for tiles
 // of 192 rows of w, which fit products of few tiles better: 2048 rows by 5120 x
@@ -1078,7 +1040,7 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
                 return;
             }
             const TileMap map = {(int)p.tiles_m, (int)p.tiles_n};
-            const int64_t blocks = std::min<int64_t>(p.tiles_m * p.tiles_n, cus);
+            const int64_t blocks = tile_blocks(p.tiles_m * p.tiles_n, cus);
             if constexpr (!g) {
                 if (p.nw == 6) {
                     out = launch(linear_tile_kernel<g, ac, 1>, blocks, 256, a8, w8, M, N, C, map, e);

@@ -1,5 +1,5 @@
 // How the FP8 product of linear.hip is computed, chosen by sizes and the
-// device's CU count; plain C++.
+// device's CU count, and which workgroup takes which tile; plain C++.
 #ifndef TANS_LINEAR_PLAN_H
 #define TANS_LINEAR_PLAN_H
 
@@ -104,6 +104,50 @@ inline Plan plan(int64_t M, int64_t N, int64_t C, bool gated, int cus) {
         p.bytes = p.splits * M * halves * p.Np * 4;
     }
     return p;
+}
+
+// Workgroups run on XCD (block % 8): a permutation of the blocks that gives each
+// XCD a run of neighbours.
+constexpr int kXcds = 8;
+constexpr int xcd_order(int block, int blocks) {
+    const int xcd = block % kXcds, per = blocks / kXcds, more = blocks % kXcds;
+    return xcd * per + (xcd < more ? xcd : more) + block / kXcds;
+}
+
+// Where a persistent workgroup's tiles lie: the tile sequence takes groups of
+// kGroupM tiles of a's rows, in each of them w's tiles in order and the group's
+// row tiles innermost; an eighth of the sequence goes to each of the 8 XCDs
+// (workgroup b runs on XCD b % 8), so that the tiles an XCD works on at a time
+// share their rows of a and w in its L2.
+constexpr int kGroupM = 8;
+
+struct TileMap {
+    int tiles_m, tiles_n;
+    constexpr int count() const { return tiles_m * tiles_n; }
+    // the i-th tile of workgroup b of `blocks`, or -1
+    constexpr int at(int i, int b, int blocks) const {
+        const int xcd = b % kXcds, T = count();
+        const int per = T / kXcds, more = T % kXcds;
+        const int first = xcd * per + (xcd < more ? xcd : more);
+        const int n = per + (xcd < more ? 1 : 0);
+        const int peers = (blocks - xcd + kXcds - 1) / kXcds;
+        const int k = i * peers + b / kXcds;
+        return k < n ? first + k : -1;
+    }
+    constexpr void place(int t, int& tm, int& tn) const {
+        const int group = t / (kGroupM * tiles_n);
+        const int m_first = group * kGroupM;
+        const int gm = tiles_m - m_first < kGroupM ? tiles_m - m_first : kGroupM;
+        const int in = t - group * kGroupM * tiles_n;
+        tm = m_first + in % gm;
+        tn = in / gm;
+    }
+};
+
+// Persistent workgroups: one a CU, and one for each eighth of the sequence that
+// holds a tile (no other workgroup takes those) on a device of fewer than 8 CUs.
+constexpr int64_t tile_blocks(int64_t tiles, int cus) {
+    return std::min<int64_t>(tiles, std::max(cus, kXcds));
 }
 
 }  // namespace tans_linear
