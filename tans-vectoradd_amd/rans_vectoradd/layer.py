@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import types
 
 import torch
 from torch.autograd import forward_ad
@@ -36,6 +37,10 @@ _BF16, _U8, _F32 = torch.bfloat16, torch.uint8, torch.float32
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
+# the level is -1 outside of dual_level; asking for a tangent takes 0.4 us there
+_forward = (forward_ad if hasattr(forward_ad, "_current_level")
+            else types.SimpleNamespace(_current_level=0))
+
 
 def _tangent(t: torch.Tensor) -> bool:
     """Whether forward-mode differentiation follows t (no_grad does not end it)."""
@@ -43,14 +48,17 @@ def _tangent(t: torch.Tensor) -> bool:
 
 
 def _ok(t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> bool:
-    # (the level is -1 outside of dual_level; unpack_dual alone takes 0.4 us)
-    return (t.dtype is dtype and t.device == dev and t.is_contiguous()
-            and not (t.requires_grad and torch.is_grad_enabled())
-            and (getattr(forward_ad, "_current_level", 0) < 0 or not _tangent(t)))
+    try:
+        return (t.dtype is dtype and t.device == dev and t.is_contiguous()
+                and not (t.requires_grad and torch.is_grad_enabled())
+                and (_forward._current_level < 0 or not _tangent(t)))
+    except AttributeError:   # no tensor
+        return False
 
 
 def _explain(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> None:
     """Raise for the first thing that keeps t from being _ok."""
+    _require(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     _check_dev(name, t, dtype)
     _require(not (t.requires_grad and torch.is_grad_enabled()),
              f"{name} requires a gradient; the layer operators have no backward")
@@ -61,6 +69,8 @@ def _explain(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) 
 
 def _rows(name: str, x: torch.Tensor, dtype: torch.dtype):
     """(M, D) of x [D] or [M, D]."""
+    if not isinstance(x, torch.Tensor):
+        _require(False, f"{name} must be a tensor")
     shape = x.shape
     if not (x.is_cuda and _ok(x, dtype, x.device) and 1 <= len(shape) <= 2
             and shape[-1] >= 16 and shape[-1] % 16 == 0):
@@ -68,6 +78,13 @@ def _rows(name: str, x: torch.Tensor, dtype: torch.dtype):
         _require(x.dim() in (1, 2), f"{name} must be [D] or [M, D]")
         _require(False, f"the columns of {name} must be a multiple of 16")
     return (1, shape[0]) if len(shape) == 1 else shape
+
+
+def _number(name: str, v) -> float:
+    try:
+        return float(v)
+    except (TypeError, ValueError, OverflowError):
+        raise RuntimeError(f"{name} must be a number") from None
 
 
 def _call(dev: torch.device, what: str, fn, *args) -> None:
@@ -92,6 +109,8 @@ def fp8_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     sum as bf16 (without residual: x itself)."""
     M, D = _rows("x", x, _BF16)
     dev, shape = x.device, x.shape
+    if type(eps) is not float:
+        eps = _number("eps", eps)
     if not (_ok(weight, _BF16, dev) and weight.shape == (D,) and eps >= 0.0):
         _explain("weight", weight, _BF16, dev)
         _require(weight.shape == (D,), f"weight must be [{D}]")
@@ -154,11 +173,13 @@ def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor | None, w: torch.Tensor,
     M, C = _rows("a", a, _U8)
     dev = a.device
     if not (_ok(w, _U8, dev) and w.dim() == 2 and w.shape[0] >= 1 and w.shape[1] == C
-            and activation in ACTIVATIONS and not (gated and w.shape[0] % 2)):
+            and isinstance(activation, str) and activation in ACTIVATIONS
+            and not (gated and w.shape[0] % 2)):
         _explain("w", w, _U8, dev)
         _require(w.dim() == 2 and w.shape[0] >= 1 and w.shape[1] == C,
                  f"w must be [R, C] with C = {C}")
-        _require(activation in ACTIVATIONS, f"activation must be one of {sorted(ACTIVATIONS)}")
+        _require(isinstance(activation, str) and activation in ACTIVATIONS,
+                 f"activation must be one of {sorted(ACTIVATIONS)}")
         _require(False, "a gated product needs an even number of rows of w")
     R = w.shape[0]
     rows = a.shape[:-1]
@@ -170,7 +191,7 @@ def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor | None, w: torch.Tensor,
             _require(False, f"w_scale must be a number or [{R}]")
         sw = w_scale.data_ptr()
     else:
-        scale = float(w_scale)
+        scale = _number("w_scale", w_scale)
     if a_scale is not None:
         if not (_ok(a_scale, _F32, dev) and a_scale.shape == rows):
             _explain("a_scale", a_scale, _F32, dev)
