@@ -358,7 +358,8 @@ int tans_fp8_quantize_rows(const void* x, int64_t M, int64_t D, void* q, float* 
  *   a          E4M3FN [M, C]; w E4M3FN [R, C]; C a multiple of 16, 16 .. 2^22,
  *              R in 1 .. 2^27 (even if gated)
  *   a_scale    float [M] or NULL (1); w_scale float [R] or NULL (1)
- *   bias       bf16 [R] or NULL; residual bf16 [M, N] or NULL
+ *   bias       bf16 [R] or NULL; residual bf16 [M, N] or NULL (either at any
+ *              multiple of 2 bytes)
  *   activation TANS_ACT_*
  *   y          bf16 [M, N]; may be residual
  *   workspace  device scratch of tans_fp8_linear_workspace's size, 16-byte

@@ -965,9 +965,11 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
         return fail(TANS_EINVAL, "linear: activation must be 0 .. 4");
     if (M == 0) return TANS_OK;
     if (!a || !w || !y) return fail(TANS_EINVAL, "linear: null pointer");
-    if (!aligned(a, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(residual, 16) ||
-        !aligned(bias, 16) || !aligned(a_scale, 4) || !aligned(w_scale, 4))
-        return fail(TANS_EINVAL, "linear: misaligned buffer (scales 4, others 16 bytes)");
+    // (bias and residual are read as rows of y are, which start anywhere if N is odd)
+    if (!aligned(a, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(residual, 2) ||
+        !aligned(bias, 2) || !aligned(a_scale, 4) || !aligned(w_scale, 4))
+        return fail(TANS_EINVAL,
+                    "linear: misaligned buffer (scales 4, bias and residual 2, others 16 bytes)");
     if (p.bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes))
         return fail(TANS_EINVAL, "linear: workspace too small, null or misaligned (16 bytes)");
     const int64_t N = gated ? R / 2 : R;
