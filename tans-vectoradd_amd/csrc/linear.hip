@@ -5,13 +5,20 @@
 //   y[m][n] = act(v[m][n]) + residual[m][n]
 //   gated: y[m][j] = act(v[m][j]) * v[m][F + j] + residual[m][j], F = R / 2
 //
-// a and w hold E4M3FN bytes, whose products are exact.  The matrix instructions
-// (v_mfma_f32_16x16x128_f8f6f4 and 32x32x64) add them in groups of 8 columns,
-// each product cut off at 2^-13 of its group's largest, and the groups in 32
-// bits; measured with sums that cancel, and alike for every FP8 form of the
-// instruction, so this is not a choice made here.  Everything after the sum is
-// 32-bit; the one rounding to fewer bits is y's to bf16, the type in which a
-// model keeps what lies between its layers.
+// a and w hold E4M3FN bytes, whose products are exact.  The FP8 matrix
+// instructions (v_mfma_f32_16x16x128_f8f6f4 and 32x32x64) add them in groups of 8
+// columns, each product cut off at 2^-13 of its group's largest, and the groups
+// in 32 bits (measured with sums that cancel, alike for every FP8 form).  The
+// bf16 instruction, to which the bytes convert exactly, cuts off at 2^-24:
+// over 4096 random columns the relative 2-norm of its error is 9e-8, as that of a
+// sum in 32 bits, and the FP8 form's 1.3e-5.  The FP8 form is the choice here:
+// its rate is 2.5 to 3 times the other's (4.4 against 1.4 .. 1.7 PFLOP/s in a loop
+// of nothing else), with half of the operands' bytes and no conversions, and y's
+// rounding to bf16, 2^-9, is a hundred times as large.  A single output whose
+// products nearly cancel can be off by several percent of itself.
+//
+// Everything after the sum is 32-bit; y is rounded once, to bf16, the type in
+// which a model keeps what lies between its layers.
 //
 // Three kernels, by what bounds them: few rows of a stream w past them (the
 // memory's rate), some rows share tiles of w (the rate at which tiles reach
@@ -35,7 +42,10 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 template <int V>
 constexpr std::integral_constant<int, V> kInt{};
 
-constexpr int64_t kMaxRows = int64_t(1) << 27;   // of w: eight rows of y stay below 2^32 bytes
+// of w: the rows of y that the lanes of a store or residual load take beside each
+// other, up to 15 of kMaxRows or, gated, 31 of half as many elements, stay within
+// 32 bits (store_staged)
+constexpr int64_t kMaxRows = int64_t(1) << 27;
 constexpr int64_t kMaxCols = int64_t(1) << 22;   // a tile's rows stay below 2^32 bytes
 
 // An offset past every tile's bytes (256 rows of kMaxCols: 2^30), also with a
@@ -385,6 +395,8 @@ __device__ __forceinline__ void store_staged(const float* stage, const Epilogue&
                                              const Residual<(GATED ? W / 2 : W), ROWS>& res,
                                              int lane, int64_t m0, int64_t M, int64_t c0, int64_t N) {
     using Res = Residual<(GATED ? W / 2 : W), ROWS>;
+    static_assert((kLanes / Res::per_row - 1) * (GATED ? kMaxRows / 2 : kMaxRows) + 64 <=
+                      (int64_t)UINT32_MAX, "`mine`, here and in Residual, in elements");
     const int p = lane % Res::per_row * 2;
     const int64_t c = c0 + p * 4;
     const uint32_t mine = (uint32_t)(lane / Res::per_row) * (uint32_t)N + p * 4;
@@ -440,16 +452,20 @@ struct MidMap {
 // linear_tile_kernel below.
 //
 // A step of 128 columns takes a workgroup 0.3 us (32 x 64 rows) to 1.2 (128 x
-// 256): its bytes reach LDS at 40 .. 46 GB/s a CU while all CUs load (11 TB/s
-// together), which takes longer than its products, so the best tile is the one
-// that covers the product in the fewest bytes a CU: 97 rows by 34816 x 5120 (gated)
-// 39.4 us with 128 x 160 (one round of 218 workgroups), 43.1 with 128 x 192,
-// 61.8 with 128 x 128 (two rounds), 62.4 with 64 x 128; 192 rows 52.4 with 192 x
-// 160, 68.0 with 256 x 256 on half of the CUs.  w is not kept in the
-// caches (non-temporal) for tiles of several rows of a: its tiles run at the
-// same time on one XCD and share it while it passes.  A product of few tiles is
-// split along its columns: 64 rows by 5120 x 17408 24.9 us in 3 parts and 37.0
-// whole, 160 by 460 x 14672 14.1 in 6 parts and 41.2.
+// 256).  Over the ten tiles that goes with the bytes that reach LDS, 40 .. 46 GB/s
+// a CU while all CUs load (11 TB/s together); the products take a SIMD 512 cycles
+// of some 2000 (1024 where two waves share it, NW > 4) and the LDS reads, 4.4
+// cycles each of 16 bytes a lane, 355 (128 x 128) to 700 (128 x 256), and nothing
+// here lays one over the other.  So the best tile is the one that covers the
+// product in the fewest bytes a CU: 97 rows by 34816 x 5120 (gated) 39.4 .. 40.7 us
+// with 128 x 160 (one round of 218 workgroups), 43.4 with 128 x 192, 61.7 with 128 x
+// 128 (two rounds), 62.3 with 64 x 128; 192 rows 52.5 with 192 x 160, 70 with 256 x
+// 256 on half of the CUs.  w is not kept in the caches (non-temporal): a tile's
+// workgroups run at the same time on one XCD and share it while it passes.  That
+// holds for a small w too, which the XCDs then fetch more than once (1003 rows by
+// 2187 x 1296: 14 MiB read of 3.9).  A product of few tiles is split along its
+// columns: 64 rows by 5120 x 17408 26.0 us in 6 parts, 33.0 in 3 and 68.6 whole; 160
+// by 460 x 14672 15.7 in 12 parts of 32 x 128 and 75.7 whole.
 //
 // With PIPE = 2 two workgroups share a CU, and one's products hide the other's
 // loads and epilogue: for products of few steps, which are mostly those
@@ -656,7 +672,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M,
 // Tiles of 256 rows of a by 256 rows of w, for products with many rows.
 //
 // Four waves of 128 x 128 outputs, 256 sums a lane, the most that the registers
-// hold: a step of 128 columns brings 64 KiB to LDS for 64 products of 32 x 32 x
+// hold: a step of 128 columns brings 64 KiB to LDS for 32 products of 32 x 32 x
 // 64 a wave.  8 waves of 64 x 128, or 16 x 16 x 128 products, read more of LDS
 // per product (8192^3 425 us with the latter, whose sums the compiler also moves
 // between registers in the loop).  Two steps lie in LDS, in units that are
@@ -665,10 +681,11 @@ __global__ __launch_bounds__(256) void linear_join_kernel(MidMap map, int64_t M,
 // 2048 of them in the matrix cores (92%).  The workgroups are persistent, so that
 // the next tile's first steps load during the epilogue.
 //
-// 8192^3 takes 369 us, 2.98 PFLOP/s; 8192 by 34816 x 5120 (gated) 1104, 2.65; 2048 by
-// 5120 x 17408 150, 2.43.  Bound by the board's power: the clock falls to 1.65 ..
+// 8192^3 takes 370 .. 400 us by the operands' values, 2.75 .. 2.98 PFLOP/s; 8192 by
+// 34816 x 5120 (gated) 1105 .. 1160 by the board, 2.52 .. 2.65; 2048 by 5120 x 17408
+// 152 .. 158, 2.3 .. 2.4.  Bound by the board's power: the clock falls to 1.65 ..
 // 1.75 GHz of 2.4 within the loop.  Besides, a tile's epilogue takes 20,000 cycles
-// in which nothing is multiplied: 17 tiles a CU by 34816 x 5120, some 15% of the
+// in which nothing is multiplied: 17 tiles a CU by 34816 x 5120, 18% of the
 // time, most of it the issue of 27 vector instructions an output.
 // ---------------------------------------------------------------------
 constexpr int kTile = 256;          // rows of either operand
@@ -678,7 +695,7 @@ constexpr int kTileWaves = 4;
 
 // GY: groups of 32 rows of w's second half that a wave takes (2, or 1 for tiles
 // of 192 rows of w, which fit products of few tiles better: 2048 rows by 5120 x
-// 17408 are 216 of them, one round at 145 us, or 160 of 256 rows at 158).
+// 17408 are 216 of them, one round at 156 us, or 160 of 256 rows at 172).
 template <bool GATED, int ACT, int GY>
 __global__ __launch_bounds__(kTileWaves * kLanes, 1) void linear_tile_kernel(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, int64_t M, int64_t N, int64_t C,

@@ -34,10 +34,10 @@ constexpr Tile kMids[] = {
     {3, 4, 0.65f, 2.0f}, {4, 4, 0.72f, 3.0f}, {4, 5, 0.88f, 3.7f}, {4, 6, 0.97f, 2.8f},
     {4, 8, 1.21f, 2.2f}, {6, 5, 1.22f, 4.3f}};
 // The large tiles: 256 rows of a by 256, or not gated 192, rows of w.  Down
-// 5120 x 17408: 2048 rows of a 158 / 145 us, 4096 334 / 290; 3000 by 5120 x
-// 5120 68 / 91, 1500 52 / 45.
+// 5120 x 17408: 2048 rows of a 172 / 156 us, 4096 350 / 305; 3000 by 5120 x
+// 5120 80 / 106, 1500 70 / 55.
 // A gated tile's epilogue takes longer (512 rows by 34816 x 5120: two rounds of
-// these 132 us, three of 128 x 192 118).
+// these 134 us, three of 128 x 192 119).
 constexpr Tile kBig = {8, 8, 1.15f, 12.0f}, kBigGated = {8, 8, 1.15f, 18.0f},
                kBig192 = {8, 6, 1.05f, 4.0f};
 constexpr float kLaunch = 4.0f, kJoin = 2.9f;        // us: a call; the second kernel
