@@ -42,16 +42,18 @@ _forward = (forward_ad if hasattr(forward_ad, "_current_level")
             else types.SimpleNamespace(_current_level=0))
 
 
-def _tangent(t: torch.Tensor) -> bool:
-    """Whether forward-mode differentiation follows t (no_grad does not end it)."""
-    return forward_ad.unpack_dual(t).tangent is not None
+def _no_tangents(**tensors) -> None:
+    """Raise for the first that forward-mode differentiation follows (no_grad does
+    not end it).  Called within a dual level only."""
+    for name, t in tensors.items():
+        _require(not isinstance(t, torch.Tensor) or forward_ad.unpack_dual(t).tangent is None,
+                 f"{name} carries a tangent; the layer operators have no forward-mode derivative")
 
 
 def _ok(t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> bool:
     try:
         return (t.dtype is dtype and t.device == dev and t.is_contiguous()
-                and not (t.requires_grad and torch.is_grad_enabled())
-                and (_forward._current_level < 0 or not _tangent(t)))
+                and not (t.requires_grad and torch.is_grad_enabled()))
     except AttributeError:   # no tensor
         return False
 
@@ -62,19 +64,19 @@ def _explain(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) 
     _check_dev(name, t, dtype)
     _require(not (t.requires_grad and torch.is_grad_enabled()),
              f"{name} requires a gradient; the layer operators have no backward")
-    _require(not _tangent(t),
-             f"{name} carries a tangent; the layer operators have no forward-mode derivative")
     _require(t.device == dev, "all tensors must be on one device")
 
 
 def _rows(name: str, x: torch.Tensor, dtype: torch.dtype):
     """(M, D) of x [D] or [M, D]."""
-    if not isinstance(x, torch.Tensor):
-        _require(False, f"{name} must be a tensor")
-    shape = x.shape
-    if not (x.is_cuda and _ok(x, dtype, x.device) and 1 <= len(shape) <= 2
-            and shape[-1] >= 16 and shape[-1] % 16 == 0):
-        _explain(name, x, dtype, x.device)
+    try:
+        shape = x.shape
+        fine = (x.is_cuda and _ok(x, dtype, x.device) and 1 <= len(shape) <= 2
+                and shape[-1] >= 16 and shape[-1] % 16 == 0)
+    except AttributeError:   # no tensor
+        fine = False
+    if not fine:
+        _explain(name, x, dtype, getattr(x, "device", None))
         _require(x.dim() in (1, 2), f"{name} must be [D] or [M, D]")
         _require(False, f"the columns of {name} must be a multiple of 16")
     return (1, shape[0]) if len(shape) == 1 else shape
@@ -109,6 +111,8 @@ def fp8_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     sum as bf16 (without residual: x itself)."""
     M, D = _rows("x", x, _BF16)
     dev, shape = x.device, x.shape
+    if _forward._current_level >= 0:
+        _no_tangents(x=x, weight=weight, residual=residual)
     if type(eps) is not float:
         eps = _number("eps", eps)
     if not (_ok(weight, _BF16, dev) and weight.shape == (D,) and eps >= 0.0):
@@ -136,6 +140,8 @@ def fp8_quantize_rows(x: torch.Tensor):
     E4M3FN(x / scale).  D a multiple of 16."""
     M, D = _rows("x", x, _BF16)
     dev = x.device
+    if _forward._current_level >= 0:
+        _no_tangents(x=x)
     q = torch.empty_like(x, dtype=_U8)
     scale = torch.empty(M if x.dim() == 2 else (), dtype=_F32, device=dev)
     _call(dev, "fp8_quantize_rows", lib.tans_fp8_quantize_rows, x.data_ptr(), M, D, q.data_ptr(),
@@ -172,6 +178,8 @@ def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor | None, w: torch.Tensor,
     its group, and the groups in 32 bits."""
     M, C = _rows("a", a, _U8)
     dev = a.device
+    if _forward._current_level >= 0:
+        _no_tangents(a_scale=a_scale, w_scale=w_scale, bias=bias, residual=residual)
     if not (_ok(w, _U8, dev) and w.dim() == 2 and w.shape[0] >= 1 and w.shape[1] == C
             and isinstance(activation, str) and activation in ACTIVATIONS
             and not (gated and w.shape[0] % 2)):
