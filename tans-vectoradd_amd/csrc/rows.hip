@@ -13,10 +13,9 @@
 // h^2 is summed from the unrounded h.  Where mean(h^2) + eps is outside 2^-100 ..
 // 2^128 (a 32-bit square has overflowed, or lost bits below 2^-126 that count),
 // the sum is taken again of h times a power of two, so that the norm of any
-// finite row is right.  The maximum is taken over the bits of
-// |y| as unsigned numbers, in which a NaN is larger than infinity: a row that
-// holds one, or an infinity, comes out with a scale that is not finite and
-// NaN bytes.
+// finite row is right.  The maximum is taken over the bits of |y| as unsigned
+// numbers, in which a NaN is larger than infinity: a row that holds one, or an
+// infinity, comes out with a scale that is not finite and NaN bytes.
 #include <algorithm>
 
 #include "layer.h"
