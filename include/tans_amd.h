@@ -377,6 +377,77 @@ int tans_fp8_linear(const void* a, const float* a_scale, const void* w, const fl
                     int32_t gated, int64_t M, int64_t R, int64_t C, void* workspace,
                     int64_t workspace_bytes, void* y, void* stream);
 
+/* ---------------- A layer's attention (no counterpart in the reference) ---
+ * Heads' elements are contiguous bf16; a token's heads lie one after the
+ * other, tokens `*_stride` elements apart (a multiple of 8, at least a row;
+ * pointers 16-byte aligned).                                             */
+
+/* Rotary positions: of every head the pairs i = 0 .. rot / 2 - 1 are turned
+ * by the angle a = positions[n] * frequencies[i] (radians) and scaled, the
+ * other elements copied:
+ *   u' = magnitude (u cos a - v sin a), v' = magnitude (u sin a + v cos a)
+ *   (u, v) = x[i], x[i + rot / 2], or interleaved x[2 i], x[2 i + 1];
+ *   inverse: by -a
+ * Angles are exact to the frequencies' last bit at any position.
+ *   x, out       bf16 [N, H, D]; out may be x (with x's stride), else they
+ *                must not overlap
+ *   positions    int32 [N]; frequencies double [rot / 2]
+ * N in 0 .. 2^30 - 1, H in 1 .. 65535, D a multiple of 16 in 16 .. 1024, rot
+ * a multiple of 16 in 16 .. D.                                           */
+int tans_rotary(const void* x, int64_t x_stride, const int32_t* positions, const double* frequencies,
+                int64_t N, int64_t H, int64_t D, int64_t rot, int32_t interleaved, int32_t inverse,
+                float magnitude, void* out, int64_t out_stride, void* stream);
+
+/* A paged cache holds [pages][heads][page][dim] rows of keys and as many of
+ * values: bf16, or E4M3FN bytes with a float scale per row ([pages][heads]
+ * [page]; NULL scales: bf16).  dim is 64, 128 or 256, page in 1 .. 2^20, fewer
+ * than 2^32 rows in all.  Slot s of sequence b is row s % page of page
+ * table[b * per + s / page].
+ *
+ * A batch of B sequences is packed into N rows: starts[b] .. starts[b + 1] - 1
+ * are sequence b's new tokens, token t of them with the slot lens[b] + t.
+ * table, starts [B + 1] and lens [B] are device memory.  No value of theirs
+ * makes an access leave the buffers: a negative length counts as 0, starts
+ * are clamped to 0 .. N; slots past the table's, and those whose entry is no
+ * page, are neither written nor seen; rows of no sequence are left as they
+ * were in the output.                                                    */
+
+/* tans_rotary of q [N, q_heads, dim] into q_out (contiguous) and of k [N,
+ * heads, dim], and k's and v's rows into the cache, 8-bit ones with
+ * scale = max(max |y|, 2^-100) / 448 and E4M3FN(y / scale) from fp32.  Every
+ * slot must be one token's.  q_heads is a multiple of heads.             */
+int tans_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                       int64_t v_stride, const int32_t* positions, const double* frequencies,
+                       int64_t rot, int32_t interleaved, float magnitude, void* k_cache, void* v_cache,
+                       float* k_scale, float* v_scale, int64_t pages, int64_t heads, int64_t page,
+                       int64_t dim, const int32_t* table, int64_t per, const int32_t* starts,
+                       const int32_t* lens, int64_t B, int64_t N, int64_t q_heads, void* q_out,
+                       void* stream);
+
+/* Attention of q [N, q_heads, dim] over the cache's heads h q_heads / heads:
+ *   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q . k_j
+ * over the slots j that the token sees: all before lens[b]; of the new
+ * ones, slot lens[b] + i, those with mask[n * mask_cols + i] (bytes 0 or 1;
+ * columns it lacks are 0), or without a mask (NULL) i <= t for token t of its
+ * sequence.  A token that sees nothing gets zeros, and what it does not see
+ * does not reach it.  Scores and sums in fp32, probabilities rounded to bf16
+ * for the product with v; a fixed order, without atomics.
+ *   scale       positive, finite
+ *   max_tokens  about the most new tokens of a sequence: chooses the kernel,
+ *               any value >= 0 is right (the same for both calls)
+ *   workspace   device scratch of tans_tree_attention_workspace's size (slots
+ *               = per * page), 16-byte aligned (contents on entry do not
+ *               matter; NULL if 0); calls that overlap in time need one each
+ *   out         bf16 [N, q_heads, dim], contiguous, not q                */
+int tans_tree_attention_workspace(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim,
+                                  int64_t slots, int64_t max_tokens, int64_t* bytes);
+int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                        const float* k_scale, const float* v_scale, int64_t pages, int64_t heads,
+                        int64_t page, int64_t dim, const int32_t* table, int64_t per,
+                        const int32_t* starts, const int32_t* lens, int64_t B, const void* mask,
+                        int64_t mask_cols, int64_t N, int64_t q_heads, float scale, int64_t max_tokens,
+                        void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,7 +33,8 @@ HIP_FLAGS = [
 # compare and a second exec mask: 6 VALU and 6 SALU per tile), so it is off
 # for kernels.hip.
 KERNEL_FLAGS = ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
-LAYER_SOURCES = ["rows", "linear"]   # norm and rounding of rows; the FP8 product
+# norm and rounding of rows; the FP8 product; rotary positions; attention
+LAYER_SOURCES = ["rows", "linear", "positions", "attention"]
 CXX_FLAGS = ["-O3", "-fPIC", "-std=c++17", "-fopenmp", "-Wall", "-Wextra"]
 
 

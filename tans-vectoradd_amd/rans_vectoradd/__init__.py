@@ -8,11 +8,19 @@ from rans_vectoradd._C import (
     fp8_vecadd_raw,
     gpu_tans_decode,
 )
+from rans_vectoradd.attention import (
+    KvCache,
+    rotary,
+    rotary_append,
+    rotary_frequencies,
+    tree_attention,
+)
 from rans_vectoradd.layer import fp8_linear, fp8_quantize_rows, fp8_rmsnorm
 from rans_vectoradd.data import QWEN3_14B_FP8_EXP, random_fp8_bytes
 from . import tans_codec
 
 __all__ = [
+    "KvCache",
     "QWEN3_14B_FP8_EXP",
     "fp8_gemm_fused_tans",
     "fp8_gemm_raw",
@@ -24,5 +32,9 @@ __all__ = [
     "fp8_vecadd_raw",
     "gpu_tans_decode",
     "random_fp8_bytes",
+    "rotary",
+    "rotary_append",
+    "rotary_frequencies",
     "tans_codec",
+    "tree_attention",
 ]

@@ -42,6 +42,10 @@ EXPORTS = (
     "tans_fp8_quantize_rows",
     "tans_fp8_linear_workspace",
     "tans_fp8_linear",
+    "tans_rotary",
+    "tans_rotary_append",
+    "tans_tree_attention_workspace",
+    "tans_tree_attention",
 )
 
 TANS_LANES = 64
@@ -101,6 +105,15 @@ for _name, _args in {
     "tans_fp8_linear_workspace": [_I64, _I64, _I64, _I32, ctypes.POINTER(_I64)],
     "tans_fp8_linear": [_P, _P, _P, _P, ctypes.c_float, _P, _P, _I32, _I32, _I64, _I64, _I64, _P,
                         _I64, _P, _P],
+    "tans_rotary": [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _I64,
+                    _P],
+    "tans_rotary_append": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I32, ctypes.c_float, _P, _P,
+                           _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _P,
+                           _P],
+    "tans_tree_attention_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                      ctypes.POINTER(_I64)],
+    "tans_tree_attention": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64,
+                            _P, _I64, _I64, _I64, ctypes.c_float, _I64, _P, _I64, _P, _P],
 }.items():
     getattr(lib, _name).restype = ctypes.c_int
     getattr(lib, _name).argtypes = _args
