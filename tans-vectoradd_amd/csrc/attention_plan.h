@@ -1,0 +1,89 @@
+// How the attention of attention.hip is computed, chosen by sizes and the device's CU
+// count, and which workgroup takes which part of the work; plain C++.
+//
+// The rows of an item are a row tile of one sequence and cache head: the new tokens'
+// query heads that read it, token by token.  A unit is 32 slots.  The work is a line of
+// pieces: sequence by sequence, in it head by head, tile by tile, unit by unit.  Split:
+// every workgroup takes an equal run of the pieces, at whose ends an item may be cut;
+// the parts of a cut item are joined by a second kernel.  Whole: a workgroup an item.
+#ifndef TANS_ATTENTION_PLAN_H
+#define TANS_ATTENTION_PLAN_H
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#ifdef __HIPCC__
+#define TANS_BOTH __host__ __device__
+#else
+#define TANS_BOTH
+#endif
+
+namespace tans_attention {
+
+constexpr int kUnit = 32;   // slots of a unit
+
+struct Work {
+    int rows;      // of a tile
+    int groups;    // workgroups, of which as many work as have `least` pieces
+    int least;
+    int whole;
+};
+
+TANS_BOTH inline int row_tiles(int64_t tokens, int64_t G, int rows) {
+    return (int)((tokens * G + rows - 1) / rows);
+}
+
+// (one at least, so that a row that sees nothing is written)
+TANS_BOTH inline int slot_units(int slots) {
+    return slots > 0 ? (int)(((int64_t)slots + kUnit - 1) / kUnit) : 1;
+}
+
+// Workgroups that share `all` pieces.
+TANS_BOTH inline int work_groups(const Work& w, int64_t all) {
+    const int64_t most = (all + w.least - 1) / w.least;
+    return (int)(most < w.groups ? most : w.groups);
+}
+
+// First piece of workgroup i < groups, and the workgroup of piece `at`: the last one
+// that starts at or before it.  (all is below 2^48: 2^30 rows' tiles of 2^26 units over
+// 65535 heads would be more, but not in any memory; groups are below 2^12.)
+TANS_BOTH inline int64_t range_start(int64_t all, int groups, int i) { return all * i / groups; }
+TANS_BOTH inline int range_of(int64_t all, int groups, int64_t at) {
+    // all i / groups <= at, so i < (at + 1) groups / all
+    return (int)(((at + 1) * groups - 1) / all);
+}
+
+// Rows of q of a tile: 32 or 64, of which each wave takes all and the waves share the
+// slots, or 128 or 256, of which each wave takes a quarter and the slots pass through
+// LDS once for all.
+enum Kind { kFew, kSome, kMany, kMost };
+struct Plan {
+    Kind kind;
+    Work work;
+    int64_t blocks, bytes;   // workgroups; of the parts
+};
+
+inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, int64_t slots,
+                 int64_t max_tokens, int cus) {
+    const int64_t G = q_heads / heads, rows = max_tokens * G;
+    Plan p = {};
+    p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome : rows <= 128 || dim == 256 ? kMany : kMost;
+    p.work.rows = 32 << p.kind;
+    // no more items than this
+    const int64_t items = (N * G / p.work.rows + std::min(N, B)) * heads;
+    p.work.least = 4;
+    p.work.whole = slots <= 8 * kUnit || (p.kind >= kMany && items >= 4 * (int64_t)cus);
+    if (p.work.whole) {
+        p.blocks = items;
+        return p;
+    }
+    p.work.groups = cus;
+    p.blocks = cus;
+    p.bytes = (int64_t)p.work.groups * 2 * p.work.rows * (dim + 2) * 4;
+    return p;
+}
+
+}  // namespace tans_attention
+
+#endif  // TANS_ATTENTION_PLAN_H
