@@ -13,11 +13,7 @@
 
 #include <algorithm>
 
-#ifdef __HIPCC__
-#define TANS_BOTH __host__ __device__
-#else
-#define TANS_BOTH
-#endif
+#include "cache_rows.h"   // TANS_BOTH
 
 namespace tans_attention {
 
@@ -30,17 +26,17 @@ struct Work {
     int whole;
 };
 
-TANS_BOTH inline int row_tiles(int64_t tokens, int64_t G, int rows) {
+TANS_BOTH int row_tiles(int64_t tokens, int64_t G, int rows) {
     return (int)((tokens * G + rows - 1) / rows);
 }
 
 // (one at least, so that a row that sees nothing is written)
-TANS_BOTH inline int slot_units(int slots) {
+TANS_BOTH int slot_units(int slots) {
     return slots > 0 ? (int)(((int64_t)slots + kUnit - 1) / kUnit) : 1;
 }
 
 // Workgroups that share `all` pieces.
-TANS_BOTH inline int work_groups(const Work& w, int64_t all) {
+TANS_BOTH int work_groups(const Work& w, int64_t all) {
     const int64_t most = (all + w.least - 1) / w.least;
     return (int)(most < w.groups ? most : w.groups);
 }
@@ -48,8 +44,8 @@ TANS_BOTH inline int work_groups(const Work& w, int64_t all) {
 // First piece of workgroup i < groups, and the workgroup of piece `at`: the last one
 // that starts at or before it.  (all is below 2^48: 2^30 rows' tiles of 2^26 units over
 // 65535 heads would be more, but not in any memory; groups are below 2^12.)
-TANS_BOTH inline int64_t range_start(int64_t all, int groups, int i) { return all * i / groups; }
-TANS_BOTH inline int range_of(int64_t all, int groups, int64_t at) {
+TANS_BOTH int64_t range_start(int64_t all, int groups, int i) { return all * i / groups; }
+TANS_BOTH int range_of(int64_t all, int groups, int64_t at) {
     // all i / groups <= at, so i < (at + 1) groups / all
     return (int)(((at + 1) * groups - 1) / all);
 }

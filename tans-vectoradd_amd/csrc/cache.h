@@ -1,16 +1,5 @@
 // The paged cache of keys and values and the packed batch that reads and writes it:
-// what positions.hip and attention.hip share.
-//
-// The cache holds `pages` pages of `page` rows for each of `heads` heads:
-// [pages][heads][page][dim], bf16, or E4M3FN bytes with a float scale per row.  A
-// page's rows of one head are contiguous, so that a head's workgroup reads runs of
-// whole pages.
-//
-// Slot s of sequence b is row s % page of page table[b][s / page].  A batch's tokens
-// are packed: rows starts[b] .. starts[b + 1] - 1 are sequence b's, and token t of
-// them has slot lens[b] + t.  These numbers lie in device memory, where the host does
-// not see them, so the kernels bound each of them: no value makes an access leave
-// the buffers.
+// what positions.hip and attention.hip share.  (Which row is whose: cache_rows.h.)
 #ifndef TANS_CACHE_H
 #define TANS_CACHE_H
 
@@ -18,55 +7,20 @@
 
 #include <string>
 
+#include "cache_rows.h"
 #include "layer.h"
 
 namespace {
 
-struct Batch {
-    const int32_t* table;    // [B][per]: pages
-    const int32_t* starts;   // [B + 1]
-    const int32_t* lens;     // [B]
-    int B, per, N;           // N: rows of q
-    uint32_t pages, heads, page;
+using tans_cache::Batch;
 
-    __device__ __forceinline__ int64_t capacity() const { return (int64_t)per * page; }
-    __device__ __forceinline__ int start(int b) const {
-        const int s = starts[b];
-        return s < 0 ? 0 : s < N ? s : N;
-    }
-    // tokens and slots before them (neither is negative; the slots within the table's)
-    __device__ __forceinline__ int tokens(int b) const {
-        const int n = start(b + 1) - start(b);
-        return n > 0 ? n : 0;
-    }
-    __device__ __forceinline__ int context(int b) const {
-        const int64_t c = lens[b];
-        return (int)(c < 0 ? 0 : c < capacity() ? c : capacity());
-    }
-    // Row of the cache (of all heads' and pages') of slot s < capacity() and head h;
-    // false if the table's entry is no page.
-    __device__ __forceinline__ bool row(int b, uint32_t s, uint32_t h, uint32_t& r) const {
-        const uint32_t i = s / page, p = (uint32_t)table[(int64_t)b * per + i];
-        r = (p * heads + h) * page + (s - i * page);
-        return p < pages;
-    }
-};
-
-// The last sequence that starts at or before row n, or -1: 64 starts are compared
-// at a time, by the lanes of a wave.
+// The last sequence that starts at or before row n, or -1.
 __device__ __forceinline__ int find_sequence(const Batch& batch, int n) {
     const int lane = threadIdx.x & (kLanes - 1);
-    int lo = 0, hi = batch.B;   // lo of them start at or before n, those from hi on do not
-    while (lo < hi) {
-        const int step = (hi - lo + kLanes - 1) / kLanes;
-        const int i = lo + (lane + 1) * step - 1;
-        const bool before = i < hi && batch.starts[i] <= n;
-        const int k = __popcll(__builtin_amdgcn_ballot_w64(before));
-        const int next = lo + k * step + step - 1;   // the first probe that is not
-        lo += k * step;
-        hi = next < hi ? next : hi;
-    }
-    return lo - 1;
+    return tans_cache::find_sequence(batch.B, [&](int lo, int step, int hi) {
+        const int64_t i = lo + (int64_t)(lane + 1) * step - 1;
+        return (int)__popcll(__builtin_amdgcn_ballot_w64(i < hi && batch.starts[i] <= n));
+    });
 }
 
 // Host side ---------------------------------------------------------------
