@@ -62,7 +62,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
 __device__ __forceinline__ int64_t cost(const Args& a, int b) {
     if (b >= a.batch.B) return 0;
     const Seq s = sequence(a, b);
-    return (int64_t)a.batch.heads * s.tiles * (a.work.whole ? 1 : s.units);
+    return (int64_t)a.batch.heads * s.tiles * (a.work.whole ? 1 : s.units + a.work.item);
 }
 
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -155,8 +155,23 @@ __device__ __forceinline__ uint32_t opaque_v(uint32_t x) {
     return x;
 }
 
-__device__ __forceinline__ float swap_halves(float v) {   // lane ^ 32's
-    return __shfl_xor(v, 32);
+// A lane's value and that of lane ^ 32, in one order for both: the swap of a register
+// with itself.  Read through a 64-bit cast: as a vector of floats that are cast back to
+// numbers the compiler has lost one of them.
+__device__ __forceinline__ uint64_t halves(uint32_t u) {
+    return __builtin_bit_cast(uint64_t, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+}
+__device__ __forceinline__ uint32_t all_bits(uint32_t u) {
+    const uint64_t p = halves(u);
+    return (uint32_t)p | (uint32_t)(p >> 32);
+}
+__device__ __forceinline__ float larger(float v) {
+    const uint64_t p = halves(__builtin_bit_cast(uint32_t, v));
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)p), __builtin_bit_cast(float, (uint32_t)(p >> 32)));
+}
+__device__ __forceinline__ float sum_of(float v) {
+    const uint64_t p = halves(__builtin_bit_cast(uint32_t, v));
+    return __builtin_bit_cast(float, (uint32_t)p) + __builtin_bit_cast(float, (uint32_t)(p >> 32));
 }
 
 __device__ __forceinline__ v16f mfma(const v8bf& a, const v8bf& b, const v16f& c) {
@@ -172,16 +187,36 @@ __device__ __forceinline__ v8bf from_fp8(uint32_t lo, uint32_t hi) {
     return __builtin_bit_cast(v8bf, u);
 }
 
-// Zero in place of infinities and NaN; whether there were any.
-__device__ __forceinline__ v8bf finite(const v8bf& x, bool& found) {
-    v4u u = __builtin_bit_cast(v4u, x);
-    #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const bool lo = (u[i] & 0x7F80u) == 0x7F80u, hi = (u[i] & 0x7F800000u) == 0x7F800000u;
-        found |= lo | hi;
-        u[i] &= (lo ? 0u : 0x0000FFFFu) | (hi ? 0u : 0xFFFF0000u);
+// Infinities and NaN among the values of a 32-bit word: join() gathers words, any() says
+// whether one of them held any, drop() puts zero in their place.
+template <bool FP8> struct Odd;
+template <> struct Odd<false> {
+    typedef uint16_t v2h __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t join(uint32_t most, uint32_t x) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2h, most),
+                                                                      __builtin_bit_cast(v2h, x & 0x7FFF7FFFu)));
     }
-    return __builtin_bit_cast(v8bf, u);
+    static __device__ __forceinline__ bool any(uint32_t most) {
+        return (most & 0xFFFFu) >= 0x7F80u || most >= 0x7F800000u;
+    }
+    static __device__ __forceinline__ uint32_t drop(uint32_t x) {
+        return x & (((x & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) | ((x & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u));
+    }
+};
+template <> struct Odd<true> {   // (the bytes 7F and FF are NaN: 7F + 1 has the top bit)
+    static __device__ __forceinline__ uint32_t join(uint32_t most, uint32_t x) {
+        return most | ((x & 0x7F7F7F7Fu) + 0x01010101u);
+    }
+    static __device__ __forceinline__ bool any(uint32_t most) { return most & 0x80808080u; }
+    static __device__ __forceinline__ uint32_t drop(uint32_t x) {
+        const uint32_t top = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+        return x & ~(top | (top - (top >> 7)));
+    }
+};
+
+// The n lowest bits, all of them or none.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1;
 }
 
 // Where a unit's rows lie in LDS: 32 rows of RB bytes, whose 16-byte pieces are
@@ -269,16 +304,20 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
             cut = false;
             left = 0;
         } else {
-            const int64_t item = in / s.units;
-            first = (int)(in - item * s.units);
+            const int pieces = s.units + a.work.item;
+            const int64_t item = in / pieces;
+            const int from = (int)(in - item * pieces);
             h = (int)(item / s.tiles);
             tile = (int)(item - (int64_t)h * s.tiles);
-            end = (int)(first + left < s.units ? first + left : s.units);
+            const int to = (int)(from + left < pieces ? from + left : pieces);
+            first = max(0, from - a.work.item);
+            end = to - a.work.item;   // (none of its units if not above first)
             is_whole = first == 0 && end == s.units;
             cut = first > 0;
-            left -= end - first;
-            in += end - first;
+            left -= to - from;
+            in += to - from;
         }
+        if (end > first) {
         const int rows = s.tokens * a.G, row0 = tile * kRows + (SHARED ? wave * 32 * RT : 0);
         // without a mask no row of the tile sees a slot past its last token's
         int seen = s.units;
@@ -306,15 +345,18 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
         }
         v16f acc[RT][D / 32];
         float m[RT], l[RT];
-        #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            m[t] = kNone;
-            l[t] = 0.0f;
+        auto clear = [&]() {
             #pragma unroll
-            for (int n = 0; n < D / 32; n++)
+            for (int t = 0; t < RT; t++) {
+                m[t] = kNone;
+                l[t] = 0.0f;
                 #pragma unroll
-                for (int c = 0; c < 16; c++) acc[t][n][c] = 0.0f;
-        }
+                for (int n = 0; n < D / 32; n++)
+                    #pragma unroll
+                    for (int c = 0; c < 16; c++) acc[t][n][c] = 0.0f;
+            }
+        };
+        clear();
 
         // The rows of unit u: looked up in the table two units before they are loaded.
         struct Lookup { uint32_t entry, off; bool in; };
@@ -332,14 +374,18 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
             const bool valid = o.in && o.entry < a.batch.pages;
             const uint32_t row = valid ? (o.entry * a.batch.heads + h) * a.batch.page + o.off : 0;
             const uint32_t exists = (uint32_t)__builtin_amdgcn_ballot_w64(valid);
+            // K's loads, then V's; the rows that a lane loads come from their lanes
+            auto of = [&](int i) { return (SHARED ? (wave * kLoads + i) % T::loads : i) * T::per_load + lane / T::pieces; };
+            constexpr int kDistinct = SHARED ? kLoads : T::loads;
+            uint32_t from[kDistinct];
+            #pragma unroll
+            for (int i = 0; i < kDistinct; i++) from[i] = __shfl(row, of(i));
             #pragma unroll
             for (int i = 0; i < kLoads; i++) {
-                const int n = SHARED ? wave * kLoads + i : i;   // of K's loads, then V's
-                const bool is_v = SHARED ? n >= T::loads : i >= T::loads;
-                const int of = (SHARED ? n % T::loads : i % T::loads) * T::per_load + lane / T::pieces;
-                const uint32_t from = __shfl(row, of);
-                const uint32_t key = is_v ? T::key_of_v(of) : T::key_of_k(of);
-                load_lds<16>((is_v ? a.v : a.k) + (int64_t)from * T::RB + ((lane % T::pieces) ^ key) * 16,
+                const int n = SHARED ? wave * kLoads + i : i;
+                const bool is_v = n >= T::loads;
+                const uint32_t at = of(i % kDistinct), key = is_v ? T::key_of_v(at) : T::key_of_k(at);
+                load_lds<16>((is_v ? a.v : a.k) + (int64_t)from[i % kDistinct] * T::RB + ((lane % T::pieces) ^ key) * 16,
                              stage + mine + n * 1024);
             }
             if constexpr (FP8)
@@ -356,16 +402,39 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
                 #pragma unroll
                 for (int c = 0; c < 16; c++) sc[t][c] = 0.0f;
             constexpr int kStep = FP8 ? 2 : 1;   // products of a read
+            constexpr int kReads = D / 16 / kStep;
+            v4u kr[kReads];
             #pragma unroll
-            for (int j = 0; j < D / 16 / kStep; j++) {
-                const v4u x = *reinterpret_cast<const v4u*>(stage + kbase[j % (kTurn / 2)] + j / (kTurn / 2) * (16 * kTurn));
+            for (int j = 0; j < kReads; j++)
+                kr[j] = *reinterpret_cast<const v4u*>(stage + kbase[j % (kTurn / 2)] + j / (kTurn / 2) * (16 * kTurn));
+            __builtin_amdgcn_sched_barrier(0);
+            #pragma unroll
+            for (int j = 0; j < kReads; j++) {
                 #pragma unroll
                 for (int e = 0; e < kStep; e++) {
-                    const v8bf kf = FP8 ? from_fp8(x[2 * e], x[2 * e + 1]) : __builtin_bit_cast(v8bf, x);
+                    const v8bf kf = FP8 ? from_fp8(kr[j][2 * e], kr[j][2 * e + 1]) : __builtin_bit_cast(v8bf, kr[j]);
                     #pragma unroll
                     for (int t = 0; t < RT; t++) sc[t] = mfma(kf, q[t][kStep * j + e], sc[t]);
                 }
             }
+            // V's operands, under way during the exponentials
+            v2u vr[D / 32][2][FP8 ? 1 : 2];
+            #pragma unroll
+            for (int n = 0; n < D / 32; n++)
+                #pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if constexpr (FP8) {
+                        typedef __attribute__((address_space(3))) v2i* P;
+                        vr[n][k][0] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                            (P)(stage + vbase[n % (kTurn / 2)] + n / (kTurn / 2) * (16 * kTurn) + k * 16 * T::RB)));
+                    } else {
+                        typedef __attribute__((address_space(3))) v4s* P;
+                        const uint8_t* from = stage + vbase[n % 2] + n / 2 * 128 + k * 16 * T::RB;
+                        vr[n][k][0] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)from));
+                        vr[n][k][1] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(from + 8 * T::RB)));
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
             float vs[FP8 ? 16 : 1];
             if constexpr (FP8) {
                 const uint8_t* scales = stage + mine + 2 * T::bytes + (SHARED ? wave * kScales : 0);
@@ -381,20 +450,29 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
                     }
                 }
             }
-            uint32_t sees[RT];
+            uint32_t sees[RT];   // the unit's slots that a row sees
             if constexpr (masked) {
+                const int before = s.context - u * kUnit;   // slots of the context
                 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    sees[t] = 0;
-                    const uint8_t* row = a.mask + (int64_t)(s.start + token[t]) * a.W;
-                    #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = i / 4 * 8 + 4 * g + i % 4, j = u * kUnit + key - s.context;
-                        bool ok = token[t] >= 0 && (exists >> key & 1);
-                        if (ok && j >= 0) ok = a.mask ? j < a.W && row[j] : j <= token[t];
-                        sees[t] |= (uint32_t)ok << key;
-                        if (!ok) sc[t][i] = kNone;
+                    sees[t] = first_bits(a.mask ? before : before + token[t] + 1);
+                    if (a.mask && before < kUnit) {
+                        // (a row's first column where the tile has none of its own)
+                        const uint8_t* row = a.mask + (int64_t)(s.start + max(token[t], 0)) * a.W;
+                        uint32_t bits = 0;
+                        #pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int key = i / 4 * 8 + 4 * g + i % 4, j = key - before;
+                            const uint32_t bit = row[j < 0 ? 0 : j < a.W ? j : a.W - 1];
+                            bits |= (j >= 0 && j < a.W ? bit : 0) << key;
+                        }
+                        sees[t] |= all_bits(bits);
                     }
+                    sees[t] = token[t] >= 0 ? sees[t] & exists : 0;
+                    const uint32_t mine = sees[t] >> 4 * g;
+                    #pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (!(mine >> (i / 4 * 8 + i % 4) & 1)) sc[t][i] = kNone;
                 }
             }
             v8bf p[RT][2];
@@ -403,7 +481,7 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
                 float top = sc[t][0];
                 #pragma unroll
                 for (int i = 1; i < 16; i++) top = fmaxf(top, sc[t][i]);
-                top = fmaxf(top, swap_halves(top));
+                top = larger(top);
                 if (__builtin_amdgcn_ballot_w64(top > m[t])) {
                     const float next = fmaxf(m[t], top);
                     const float by = next == kNone ? 0.0f : __builtin_amdgcn_exp2f((m[t] - next) * a.c);
@@ -421,7 +499,7 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
                     e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], a.c, -mc));
                     l[t] += e[i];
                     // (what is not seen may have any scale)
-                    if constexpr (FP8) e[i] = masked && sc[t][i] == kNone ? 0.0f : e[i] * vs[i];
+                    if constexpr (FP8) e[i] = masked && e[i] == 0.0f ? 0.0f : e[i] * vs[i];
                 }
                 #pragma unroll
                 for (int k = 0; k < 2; k++)
@@ -430,37 +508,41 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
                                                           bf16_pack(e[8 * k + 4], e[8 * k + 5]),
                                                           bf16_pack(e[8 * k + 6], e[8 * k + 7])});
             }
-            bool odd = false;
+            // A value that is infinite or NaN reaches the rows that see its slot, and by the
+            // matrix product it would reach the others as well (0 times it is NaN): it is
+            // left out there, and added below.
+            uint64_t odd = 0;
+            if constexpr (masked) {
+                uint32_t most = 0;
+                #pragma unroll
+                for (int n = 0; n < D / 32; n++)
+                    #pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        #pragma unroll
+                        for (int w = 0; w < (FP8 ? 2 : 4); w++) most = Odd<FP8>::join(most, vr[n][k][w / 2][w % 2]);
+                odd = __builtin_amdgcn_ballot_w64(Odd<FP8>::any(most));
+                if (odd) {
+                    #pragma unroll
+                    for (int n = 0; n < D / 32; n++)
+                        #pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            #pragma unroll
+                            for (int w = 0; w < (FP8 ? 2 : 4); w++) vr[n][k][w / 2][w % 2] = Odd<FP8>::drop(vr[n][k][w / 2][w % 2]);
+                }
+            }
             #pragma unroll
             for (int n = 0; n < D / 32; n++) {
                 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    v8bf vf;
-                    if constexpr (FP8) {
-                        typedef __attribute__((address_space(3))) v2i* P;
-                        const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                            (P)(stage + vbase[n % (kTurn / 2)] + n / (kTurn / 2) * (16 * kTurn) + k * 16 * T::RB));
-                        vf = from_fp8((uint32_t)x[0], (uint32_t)x[1]);
-                    } else {
-                        typedef __attribute__((address_space(3))) v4s* P;
-                        const uint8_t* at = stage + vbase[n % 2] + n / 2 * 128 + k * 16 * T::RB;
-                        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at);
-                        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 8 * T::RB));
-                        const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
-                        vf = __builtin_bit_cast(v8bf, v4u{xu[0], xu[1], yu[0], yu[1]});
-                    }
-                    if constexpr (masked) vf = finite(vf, odd);
+                    const v2u* x = vr[n][k];
+                    const v8bf vf = FP8 ? from_fp8(x[0][0], x[0][1])
+                                  : __builtin_bit_cast(v8bf, v4u{x[0][0], x[0][1], x[FP8 ? 0 : 1][0], x[FP8 ? 0 : 1][1]});
                     #pragma unroll
                     for (int t = 0; t < RT; t++) acc[t][n] = mfma(vf, p[t][k], acc[t][n]);
                 }
             }
             if constexpr (masked) {
-                // A value that is infinite or NaN reaches the rows that see its slot, and
-                // by the matrix product it would reach the others as well (0 times it is
-                // NaN): it was left out there, and is added here.
-                if (__builtin_amdgcn_ballot_w64(odd)) {
-                    #pragma unroll
-                    for (int t = 0; t < RT; t++) sees[t] |= __shfl_xor(sees[t], 32);
+                if (odd) {
                     for (uint32_t key = 0; key < kUnit; key++) {
                         const uint8_t* row = stage + mine + T::bytes + key * T::RB + g * (FP8 ? 4 : 8);
                         const uint32_t by = T::key_of_v(key);
@@ -491,73 +573,83 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
             }
         };
 
-        // A wave's units: every one, or the NW-th from its own on.  Up to `plain` every
-        // row sees all of a unit's slots, if they exist.
+
+        // A wave's units: every one, or the NW-th from its own on.  Below `plain` every row
+        // sees all of a unit's slots, if they exist.
         constexpr int kBy = SHARED ? 1 : NW;
-        const int plain = (int)(((int64_t)s.context + (a.mask ? 0 : tile * kRows / a.G + 1)) / kUnit);
-        int u = first + (SHARED ? 0 : wave), now = 0;
-        uint32_t exists[STAGES];
+        const int plain = min(stop, (int)(((int64_t)s.context + (a.mask ? 0 : tile * kRows / a.G + 1)) / kUnit));
+        const int u0 = first + (SHARED ? 0 : wave);
         uint8_t* const rings[4] = {ring0, ring1, ring2, ring3};
-        Lookup la = look_up(u), lb = look_up(u + kBy);
-        auto fetch = [&](int v, uint8_t* stage) {   // unit v, whose lookup is la
+        uint32_t exists[STAGES];
+        Lookup la, lb;
+        auto fetch = [&](int v, int i) {   // unit v, whose lookup is la, into stage i
             const Lookup l = la;
             la = lb;
             lb = look_up(v + 2 * kBy);
-            return issue(l, stage);
+            exists[i] = issue(l, rings[i]);
         };
         constexpr int kAhead = SHARED ? STAGES - 1 : STAGES;   // units under way
-        #pragma unroll
-        for (int i = 0; i < kAhead; i++) exists[i] = fetch(u + i * kBy, rings[i]);
-        // One unit in ring `i`; false, and its place in `now`, if it is not a plain one.
-        auto step = [&](int i) {
-            if constexpr (SHARED) arrive<(kAhead - 1) * kIssue>(); else wait_loads<(kAhead - 1) * kIssue>();
-            const int w = __builtin_amdgcn_readfirstlane(u);
-            if (w >= plain || w >= stop || exists[i] != 0xFFFFFFFFu) {
-                now = i;
-                return false;
-            }
-            // shared: refilled is the stage that all waves have read before the barrier
-            if constexpr (SHARED) exists[(i + kAhead) % STAGES] = fetch(u + kAhead, rings[(i + kAhead) % STAGES]);
-            compute(std::false_type{}, u, exists[i], rings[i]);
-            if constexpr (!SHARED) {
-                // (the reads of this stage have come: the products have used them)
-                __builtin_amdgcn_sched_barrier(0);
-                asm volatile("" ::: "memory");
-                exists[i] = fetch(u + STAGES * kBy, rings[i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            u += kBy;
-            return true;
+        auto begin = [&](int v) {
+            la = look_up(v);
+            lb = look_up(v + kBy);
+            #pragma unroll
+            for (int i = 0; i < kAhead; i++) fetch(v + i * kBy, i);
         };
-        while (true) {
-            if (!step(0)) break;
-            if (!step(1)) break;
-            if (STAGES > 2 && !step(2)) break;
-            if (STAGES > 3 && !step(3)) break;
+        begin(u0);
+        // Plain units, a round of the stages at a time (an exit between two stages would
+        // make the compiler wait for all loads in each).
+        int u = u0;
+        uint32_t whole = 0xFFFFFFFFu;
+        while (u + (STAGES - 1) * kBy < plain) {
+            #pragma unroll
+            for (int i = 0; i < STAGES; i++) {
+                if constexpr (SHARED) {
+                    arrive<(kAhead - 1) * kIssue>();
+                    whole &= exists[i];
+                    // (the stage that all waves have read before the barrier)
+                    fetch(u + kAhead, (i + kAhead) % STAGES);
+                    compute(std::false_type{}, u, 0, rings[i]);
+                } else {
+                    wait_loads<(kAhead - 1) * kIssue>();
+                    whole &= exists[i];
+                    compute(std::false_type{}, u, 0, rings[i]);
+                    // (the reads of this stage have come: the products have used them)
+                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" ::: "memory");
+                    fetch(u + STAGES * kBy, i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                u += kBy;
+            }
         }
-        // The others: kAhead units lie in the stages from `now` on.
+        if (__builtin_amdgcn_readfirstlane(whole) != 0xFFFFFFFFu) {
+            // some of them were of pages that do not exist: all over again, slot by slot
+            if constexpr (SHARED) arrive<0>(); else wait_loads<0>();
+            clear();
+            u = u0;
+            begin(u);
+        }
+        // The others: kAhead units lie in the stages from the first on.
         while (true) {
             if constexpr (SHARED) arrive<0>(); else wait_loads<0>();
             for (int i = 0; i < kAhead && u < stop; i++, u += kBy) {
-                uint8_t* stage = now == 0 ? ring0 : now == 1 ? ring1 : now == 2 ? ring2 : ring3;
+                const uint8_t* stage = i == 0 ? ring0 : i == 1 ? ring1 : i == 2 ? ring2 : ring3;
                 uint32_t e = exists[0];
                 #pragma unroll
-                for (int k = 1; k < STAGES; k++) e = now == k ? exists[k] : e;
+                for (int k = 1; k < kAhead; k++) e = i == k ? exists[k] : e;
                 compute(std::true_type{}, u, e, stage);
-                now = now + 1 == STAGES ? 0 : now + 1;
             }
             if (u >= stop) break;
             if constexpr (SHARED) arrive<0>();
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
-            now = 0;
             #pragma unroll
-            for (int i = 0; i < kAhead; i++) exists[i] = fetch(u + i * kBy, rings[i]);
+            for (int i = 0; i < kAhead; i++) fetch(u + i * kBy, i);
         }
         if constexpr (SHARED) arrive<0>();   // (before the ring is filled again)
 
         #pragma unroll
-        for (int t = 0; t < RT; t++) l[t] += swap_halves(l[t]);
+        for (int t = 0; t < RT; t++) l[t] = sum_of(l[t]);
         const bool to_parts = !is_whole;
         const int64_t slot = (int64_t)blockIdx.x * 2 + (cut ? 0 : 1);
         float* part_o = a.parts + slot * kRows * D;
@@ -650,8 +742,9 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
             }
             if (left > 0) __syncthreads();   // (before the ring is filled again)
         }
+        }
         // the next item's sequence
-        if (left > 0 && in == (int64_t)a.batch.heads * s.tiles * s.units) {
+        if (left > 0 && in == (int64_t)a.batch.heads * s.tiles * (s.units + a.work.item)) {
             in = 0;
             do {
                 if (++b == a.batch.B) return;   // (not reached while nobody writes to the batch)
@@ -677,7 +770,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
     const int groups = work_groups(a.work, all);
     const int h = hq / a.G, row = (n - s.start) * a.G + hq % a.G;
     const int tile = row / a.work.rows, local = row % a.work.rows;
-    const int64_t from = before + ((int64_t)h * s.tiles + tile) * s.units, to = from + s.units;
+    const int64_t from = before + ((int64_t)h * s.tiles + tile) * (s.units + a.work.item) + a.work.item,
+                  to = from + s.units;
     const int w0 = range_of(all, groups, from), w1 = range_of(all, groups, to - 1);
     if (w0 == w1) return;   // (one workgroup had the whole item)
     constexpr int E = D / kLanes;

@@ -23,6 +23,7 @@ struct Work {
     int rows;      // of a tile
     int groups;    // workgroups, of which as many work as have `least` pieces
     int least;
+    int item;      // pieces that an item counts besides its units
     int whole;
 };
 
@@ -68,7 +69,8 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
     p.work.rows = 32 << p.kind;
     // no more items than this
     const int64_t items = (N * G / p.work.rows + std::min(N, B)) * heads;
-    p.work.least = 4;
+    p.work.least = 8;
+    p.work.item = 8;
     p.work.whole = slots <= 8 * kUnit || (p.kind >= kMany && items >= 4 * (int64_t)cus);
     if (p.work.whole) {
         p.blocks = items;
