@@ -117,11 +117,18 @@ __device__ __forceinline__ int find_piece(const Args& a, int64_t& at) {
     return a.batch.B - 1;   // (not reached)
 }
 
+// LDS is addressed by pointers of its own address space: a plain pointer to it that the
+// compiler keeps in a table and loads from there it takes for one to memory.
+#define TANS_LDS __attribute__((address_space(3)))
+typedef TANS_LDS uint8_t* Lds;
+template <class V>
+__device__ __forceinline__ V lds_read(Lds from) { return *(const TANS_LDS V*)from; }
+
 // 16 or 4 bytes a lane from memory to LDS, lane l's to lds + 16 l or 4 l.
 template <int BYTES>
-__device__ __forceinline__ void load_lds(const void* from, uint8_t* to) {
+__device__ __forceinline__ void load_lds(const void* from, Lds to) {
     const auto* p = (const __attribute__((address_space(1))) void*)from;
-    auto* lds = (__attribute__((address_space(3))) void*)to;
+    auto* lds = (TANS_LDS void*)to;
     if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(p, lds, 16, 0, 0);
     else __builtin_amdgcn_global_load_lds(p, lds, 4, 0, 0);
 }
@@ -236,522 +243,827 @@ struct Tile {
     }
 };
 
-// 32 slots at a time.  S^T = K Q^T by 32 x 32 x 16 products: lane (g, r), lane 32 g +
-// r, gets query row r's scores with the slots 8 i + 4 g + c (i, c = 0 .. 3), so that a
-// row's maximum and sum are one lane's and its other half's.  Those 16 are, rounded to
-// bf16, the operand of O^T = V^T P^T as they lie there, if the slots are taken in that
-// order; V's operand, 8 slots of one dimension, comes from LDS by transposing reads.
-template <int D, bool FP8, int RT, bool SHARED, int NW, int STAGES>
-__global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
+// Where a lane finds its operands in a stage: K's (slots x dimensions) and V's.
+template <int D, bool FP8>
+struct Places {
     using T = Tile<D, FP8>;
-    constexpr int kRows = 32 * RT * (SHARED ? NW : 1);
-    constexpr int kShare = SHARED ? NW : 1;               // waves that share a tile
-    constexpr int kLoads = 2 * T::loads / kShare;         // of a wave and unit
-    static_assert(2 * T::loads % kShare == 0, "loads");
-    constexpr int kIssue = kLoads + (FP8 ? 1 : 0);        // with the scales'
-    constexpr int kScales = FP8 ? 256 : 0;
-    constexpr int kStage = 2 * T::bytes + kScales * (SHARED ? NW : 1);
-    constexpr int kRing = kStage * (SHARED ? 1 : NW);
-    __shared__ __attribute__((aligned(1024))) uint8_t ring0[kRing], ring1[kRing],
-        ring2[STAGES > 2 ? kRing : 16], ring3[STAGES > 3 ? kRing : 16];
-    __shared__ float stat[SHARED ? 1 : NW][kRows][2];
-    const int lane = threadIdx.x & (kLanes - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-    const int r = lane & 31, g = lane >> 5;
-
-    int64_t all, none;
-    total_cost(a, 0, all, none);
-    const int groups = a.work.whole ? 0 : work_groups(a.work, all);
-    if (a.work.whole ? (int64_t)blockIdx.x >= all : (int)blockIdx.x >= groups) return;
-    int64_t at = a.work.whole ? (int64_t)blockIdx.x : range_start(all, groups, blockIdx.x);
-    int64_t left = a.work.whole ? 1 : range_start(all, groups, blockIdx.x + 1) - at;
-    int64_t in = at;   // the piece's number in its sequence
-    int b = find_piece(a, in);
-    Seq s = sequence(a, b);
-
-    // addresses in a stage, of K's and V's operands
-    const uint32_t mine = SHARED ? 0 : wave * kStage;
-    uint32_t kbase[4], vbase[4];
-    #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        kbase[i] = opaque_v(mine + r * T::RB + (((2 * i + g) ^ T::key_of_k(r)) % T::pieces) * 16);
-        const int l = lane & 15, half = (lane >> 4) & 1;
-        if constexpr (FP8) {
-            const uint32_t row = l / 2 < 4 ? 4 * g + l / 2 : 4 + 4 * g + l / 2;
-            vbase[i] = opaque_v(mine + T::bytes + row * T::RB +
-                                (((2 * i + half) ^ T::key_of_v(row)) % T::pieces) * 16 + l % 2 * 8);
-        } else {
-            const uint32_t row = 4 * g + l / 4;
-            vbase[i] = opaque_v(mine + T::bytes + row * T::RB +
-                                (((4 * (i & 1) + 2 * half + l % 4 / 2) ^ T::key_of_v(row)) % T::pieces) * 16 +
-                                l % 2 * 8);
+    static constexpr int turn = T::pieces < 8 ? 4 : 8;   // pieces of a row that the keys permute
+    uint32_t k[4], v[4];
+    __device__ __forceinline__ void set(int lane) {
+        const int r = lane & 31, g = lane >> 5, l = lane & 15, half = (lane >> 4) & 1;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            k[i] = opaque_v(r * T::RB + (((2 * i + g) ^ T::key_of_k(r)) % T::pieces) * 16);
+            if constexpr (FP8) {
+                const uint32_t row = l / 2 < 4 ? 4 * g + l / 2 : 4 + 4 * g + l / 2;
+                v[i] = opaque_v(T::bytes + row * T::RB + (((2 * i + half) ^ T::key_of_v(row)) % T::pieces) * 16 + l % 2 * 8);
+            } else {
+                const uint32_t row = 4 * g + l / 4;
+                v[i] = opaque_v(T::bytes + row * T::RB +
+                                (((4 * (i & 1) + 2 * half + l % 4 / 2) ^ T::key_of_v(row)) % T::pieces) * 16 + l % 2 * 8);
+            }
         }
     }
-    // pieces of a row that the keys permute: 8, or 4
-    constexpr int kTurn = T::pieces < 8 ? 4 : 8;
-
-    while (left > 0) {
-        // the item: row tile `tile` of cache head h, units first .. end - 1 of it
-        int h, tile, first, end;
-        bool is_whole;
-        bool cut;    // it began in another workgroup's run
-        if (a.work.whole) {
-            h = (int)(in % a.batch.heads);
-            tile = s.tiles - 1 - (int)(in / a.batch.heads);
-            first = 0;
-            end = s.units;
-            is_whole = true;
-            cut = false;
-            left = 0;
+    // operand j of K: 8 dimensions of slot r, those that load_query gives product j (of 8
+    // bits j and j + 1, j even)
+    __device__ __forceinline__ v4u read_k(Lds stage, int j) const {
+        const int i = FP8 ? j / 2 : j;
+        return lds_read<v4u>(stage + k[i % (turn / 2)] + i / (turn / 2) * (16 * turn));
+    }
+    // operand of V for dimensions 32 n .. 32 n + 31 and half h of the slots
+    __device__ __forceinline__ v4u read_v(Lds stage, int n, int h) const {
+        if constexpr (FP8) {
+            typedef TANS_LDS v2i* P;
+            const v2u x = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (P)(stage + v[n % (turn / 2)] + n / (turn / 2) * (16 * turn) + h * 16 * T::RB)));
+            return v4u{x[0], x[1], 0, 0};
         } else {
-            const int pieces = s.units + a.work.item;
-            const int64_t item = in / pieces;
-            const int from = (int)(in - item * pieces);
-            h = (int)(item / s.tiles);
-            tile = (int)(item - (int64_t)h * s.tiles);
-            const int to = (int)(from + left < pieces ? from + left : pieces);
-            first = max(0, from - a.work.item);
-            end = to - a.work.item;   // (none of its units if not above first)
-            is_whole = first == 0 && end == s.units;
-            cut = first > 0;
-            left -= to - from;
-            in += to - from;
+            typedef TANS_LDS v4s* P;
+            const Lds from = stage + v[n % 2] + n / 2 * 128 + h * 16 * T::RB;
+            const v2u x = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)from));
+            const v2u y = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(from + 8 * T::RB)));
+            return v4u{x[0], x[1], y[0], y[1]};
         }
-        if (end > first) {
-        const int rows = s.tokens * a.G, row0 = tile * kRows + (SHARED ? wave * 32 * RT : 0);
-        // without a mask no row of the tile sees a slot past its last token's
-        int seen = s.units;
-        if (!a.mask) {
-            const int last = min(s.tokens - 1, (tile * kRows + kRows - 1) / a.G);
-            seen = slot_units((int)min((int64_t)s.slots, (int64_t)s.context + last + 1));
-        }
-        const int stop = end < seen ? end : seen;
+    }
+};
 
-        v8bf q[RT][D / 16];
-        int token[RT];
+// A tile's 32 rows of q, lane (g, r) holding row r's operands.
+template <int D, bool FP8>
+__device__ __forceinline__ void load_query(const Args& a, const uint16_t* p, bool exists, v8bf (&q)[D / 16]) {
+    const int g = (threadIdx.x & (kLanes - 1)) >> 5;
+    #pragma unroll
+    for (int j = 0; j < D / 16; j++) {
+        v4u u = {0, 0, 0, 0};
+        if (exists) u = *reinterpret_cast<const v4u*>(p + (FP8 ? j / 2 * 32 + 16 * g + j % 2 * 8 : 16 * j + 8 * g));
+        q[j] = __builtin_bit_cast(v8bf, u);
+    }
+}
+
+// The running sums of 32 rows: lane (g, r) has row r's dimensions 32 n + 8 i + 4 g + c in
+// acc[n][4 i + c], its maximum, and of its sum the part of its own slots.
+//
+// The maximum is one that exponents refer to, not the largest score: it is raised, and
+// the sums brought to it, when a score exceeds it by more than 2^kLoose in the
+// probability.  That keeps the factor of D values out of all but a few units, and costs
+// no bits: probabilities are rounded to bf16 whatever their exponent, sums are 32 bits'.
+constexpr float kLoose = 8.0f;
+template <int D>
+struct Sums {
+    v16f acc[D / 32];
+    float m, l;
+    __device__ __forceinline__ void clear() {
+        m = kNone;
+        l = 0.0f;
         #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int row = row0 + 32 * t + r;
-            token[t] = row < rows ? row / a.G : -1;
-            const uint16_t* p = a.q + (int64_t)(s.start + token[t]) * a.q_stride +
-                                (int64_t)(h * a.G + row % a.G) * D;
+        for (int n = 0; n < D / 32; n++)
             #pragma unroll
-            for (int j = 0; j < D / 16; j++) {
-                v4u u = {0, 0, 0, 0};
-                if (row < rows)
-                    u = *reinterpret_cast<const v4u*>(p + (FP8 ? j / 2 * 32 + 16 * g + j % 2 * 8 : 16 * j + 8 * g));
-                q[t][j] = __builtin_bit_cast(v8bf, u);
-            }
-        }
-        v16f acc[RT][D / 32];
-        float m[RT], l[RT];
-        auto clear = [&]() {
-            #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                m[t] = kNone;
-                l[t] = 0.0f;
-                #pragma unroll
-                for (int n = 0; n < D / 32; n++)
-                    #pragma unroll
-                    for (int c = 0; c < 16; c++) acc[t][n][c] = 0.0f;
-            }
-        };
-        clear();
-
-        // The rows of unit u: looked up in the table two units before they are loaded.
-        struct Lookup { uint32_t entry, off; bool in; };
-        auto look_up = [&](int u) {
-            const uint32_t slot = (uint32_t)u * kUnit + r;
-            Lookup o;
-            o.in = u < stop && slot < (uint32_t)s.slots;
-            const uint32_t i = o.in ? slot / a.batch.page : 0;
-            o.off = slot - i * a.batch.page;
-            o.entry = s.slots > 0 ? (uint32_t)a.batch.table[(int64_t)b * a.batch.per + i] : 0;
-            return o;
-        };
-        // loads unit's rows (of nothing: row 0's, which no lane sees); the slots that exist
-        auto issue = [&](const Lookup& o, uint8_t* stage) {
-            const bool valid = o.in && o.entry < a.batch.pages;
-            const uint32_t row = valid ? (o.entry * a.batch.heads + h) * a.batch.page + o.off : 0;
-            const uint32_t exists = (uint32_t)__builtin_amdgcn_ballot_w64(valid);
-            // K's loads, then V's; the rows that a lane loads come from their lanes
-            auto of = [&](int i) { return (SHARED ? (wave * kLoads + i) % T::loads : i) * T::per_load + lane / T::pieces; };
-            constexpr int kDistinct = SHARED ? kLoads : T::loads;
-            uint32_t from[kDistinct];
-            #pragma unroll
-            for (int i = 0; i < kDistinct; i++) from[i] = __shfl(row, of(i));
-            #pragma unroll
-            for (int i = 0; i < kLoads; i++) {
-                const int n = SHARED ? wave * kLoads + i : i;
-                const bool is_v = n >= T::loads;
-                const uint32_t at = of(i % kDistinct), key = is_v ? T::key_of_v(at) : T::key_of_k(at);
-                load_lds<16>((is_v ? a.v : a.k) + (int64_t)from[i % kDistinct] * T::RB + ((lane % T::pieces) ^ key) * 16,
-                             stage + mine + n * 1024);
-            }
-            if constexpr (FP8)
-                load_lds<4>((g ? a.v_scale : a.k_scale) + row,
-                            stage + mine + 2 * T::bytes + (SHARED ? wave * kScales : 0));
-            return exists;
-        };
-
-        auto compute = [&](auto MASKED, int u, uint32_t exists, const uint8_t* stage) {
-            constexpr bool masked = decltype(MASKED)::value;
-            v16f sc[RT];
-            #pragma unroll
-            for (int t = 0; t < RT; t++)
-                #pragma unroll
-                for (int c = 0; c < 16; c++) sc[t][c] = 0.0f;
-            constexpr int kStep = FP8 ? 2 : 1;   // products of a read
-            constexpr int kReads = D / 16 / kStep;
-            v4u kr[kReads];
-            #pragma unroll
-            for (int j = 0; j < kReads; j++)
-                kr[j] = *reinterpret_cast<const v4u*>(stage + kbase[j % (kTurn / 2)] + j / (kTurn / 2) * (16 * kTurn));
-            __builtin_amdgcn_sched_barrier(0);
-            #pragma unroll
-            for (int j = 0; j < kReads; j++) {
-                #pragma unroll
-                for (int e = 0; e < kStep; e++) {
-                    const v8bf kf = FP8 ? from_fp8(kr[j][2 * e], kr[j][2 * e + 1]) : __builtin_bit_cast(v8bf, kr[j]);
-                    #pragma unroll
-                    for (int t = 0; t < RT; t++) sc[t] = mfma(kf, q[t][kStep * j + e], sc[t]);
-                }
-            }
-            // V's operands, under way during the exponentials
-            v2u vr[D / 32][2][FP8 ? 1 : 2];
+            for (int c = 0; c < 16; c++) acc[n][c] = 0.0f;
+    }
+    // Admits a unit's scores; returns what to take from score * c in the exponent.
+    __device__ __forceinline__ float admit(const v16f& sc, float c) {
+        float top = sc[0];
+        #pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, sc[i]);
+        top = larger(top);
+        // (where m is kNone any score but that one exceeds it; NaN has no part in top)
+        if (__builtin_amdgcn_ballot_w64((top - m) * c > kLoose)) {
+            const float next = fmaxf(m, top);
+            const float by = next == kNone ? 0.0f : __builtin_amdgcn_exp2f((m - next) * c);
+            m = next;
+            l *= by;
             #pragma unroll
             for (int n = 0; n < D / 32; n++)
                 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    if constexpr (FP8) {
-                        typedef __attribute__((address_space(3))) v2i* P;
-                        vr[n][k][0] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                            (P)(stage + vbase[n % (kTurn / 2)] + n / (kTurn / 2) * (16 * kTurn) + k * 16 * T::RB)));
-                    } else {
-                        typedef __attribute__((address_space(3))) v4s* P;
-                        const uint8_t* from = stage + vbase[n % 2] + n / 2 * 128 + k * 16 * T::RB;
-                        vr[n][k][0] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)from));
-                        vr[n][k][1] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(from + 8 * T::RB)));
-                    }
-                }
-            __builtin_amdgcn_sched_barrier(0);
-            float vs[FP8 ? 16 : 1];
-            if constexpr (FP8) {
-                const uint8_t* scales = stage + mine + 2 * T::bytes + (SHARED ? wave * kScales : 0);
-                #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const v4f ks = *reinterpret_cast<const v4f*>(scales + (8 * i + 4 * g) * 4);
-                    const v4f vi = *reinterpret_cast<const v4f*>(scales + 128 + (8 * i + 4 * g) * 4);
-                    #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        vs[4 * i + c] = vi[c];
-                        #pragma unroll
-                        for (int t = 0; t < RT; t++) sc[t][4 * i + c] *= ks[c];
-                    }
-                }
-            }
-            uint32_t sees[RT];   // the unit's slots that a row sees
-            if constexpr (masked) {
-                const int before = s.context - u * kUnit;   // slots of the context
-                #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    sees[t] = first_bits(a.mask ? before : before + token[t] + 1);
-                    if (a.mask && before < kUnit) {
-                        // (a row's first column where the tile has none of its own)
-                        const uint8_t* row = a.mask + (int64_t)(s.start + max(token[t], 0)) * a.W;
-                        uint32_t bits = 0;
-                        #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = i / 4 * 8 + 4 * g + i % 4, j = key - before;
-                            const uint32_t bit = row[j < 0 ? 0 : j < a.W ? j : a.W - 1];
-                            bits |= (j >= 0 && j < a.W ? bit : 0) << key;
-                        }
-                        sees[t] |= all_bits(bits);
-                    }
-                    sees[t] = token[t] >= 0 ? sees[t] & exists : 0;
-                    const uint32_t mine = sees[t] >> 4 * g;
-                    #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (!(mine >> (i / 4 * 8 + i % 4) & 1)) sc[t][i] = kNone;
-                }
-            }
-            v8bf p[RT][2];
+                for (int i = 0; i < 16; i++) acc[n][i] *= by;
+        }
+        return m == kNone ? 0.0f : m * c;
+    }
+};
+
+// The scales of a lane's 16 slots: 8 i + 4 g + c for value 4 i + c.
+__device__ __forceinline__ void read_scales(Lds from, float (&f)[16]) {
+    const int g = (threadIdx.x & (kLanes - 1)) >> 5;
+    #pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const v4f x = lds_read<v4f>(from + (8 * i + 4 * g) * 4);
+        #pragma unroll
+        for (int c = 0; c < 4; c++) f[4 * i + c] = x[c];
+    }
+}
+
+// A unit for 32 rows.  S^T = K Q^T by 32 x 32 x 16 products: lane (g, r), lane 32 g + r,
+// gets query row r's scores with the slots 8 i + 4 g + c (i, c = 0 .. 3), so that a row's
+// maximum and sum are one lane's and its other half's.  Those 16 are, rounded to bf16,
+// the operand of O^T = V^T P^T as they lie there, if the slots are taken in that order;
+// V's operand, 8 slots of one dimension, comes from LDS by transposing reads.
+struct Mask {
+    int token;         // the lane's row's, in its sequence, or -1
+    int start;         // the sequence's first row of q
+    int before;        // slots of the context from the unit's first on
+    uint32_t exists;   // of the unit's slots
+};
+template <int D, bool FP8, bool MASKED>
+__device__ __forceinline__ void attend_unit(const Args& a, const Places<D, FP8>& at, Lds stage, Lds scales,
+                                            const v8bf (&q)[D / 16], Sums<D>& sums,
+                                            const Mask& mask) {
+    using T = Tile<D, FP8>;
+    const int lane = threadIdx.x & (kLanes - 1), g = lane >> 5;
+    v16f sc;
+    #pragma unroll
+    for (int c = 0; c < 16; c++) sc[c] = 0.0f;
+    constexpr int kStep = FP8 ? 2 : 1;   // products of a read
+    v4u kr[D / 16 / kStep];
+    #pragma unroll
+    for (int j = 0; j < D / 16; j += kStep) kr[j / kStep] = at.read_k(stage, j);
+    __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+    for (int j = 0; j < D / 16; j++) {
+        const v4u& x = kr[j / kStep];
+        sc = mfma(FP8 ? from_fp8(x[2 * (j % 2)], x[2 * (j % 2) + 1]) : __builtin_bit_cast(v8bf, x), q[j], sc);
+    }
+    // V's operands, under way during the exponentials
+    v4u vr[D / 32][2];
+    #pragma unroll
+    for (int n = 0; n < D / 32; n++)
+        #pragma unroll
+        for (int k = 0; k < 2; k++) vr[n][k] = at.read_v(stage, n, k);
+    __builtin_amdgcn_sched_barrier(0);
+    float vs[16];
+    if constexpr (FP8) {
+        float ks[16];
+        read_scales(scales, ks);
+        read_scales(scales + 128, vs);
+        #pragma unroll
+        for (int i = 0; i < 16; i++) sc[i] *= ks[i];
+    }
+    uint32_t sees = 0xFFFFFFFFu;   // the unit's slots that the row sees
+    if constexpr (MASKED) {
+        sees = first_bits(a.mask ? mask.before : mask.before + mask.token + 1);
+        if (a.mask && mask.before < kUnit) {
+            // (a row's first column where the tile has none of its own)
+            const uint8_t* row = a.mask + (int64_t)(mask.start + max(mask.token, 0)) * a.W;
+            uint32_t bits = 0;
             #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                float top = sc[t][0];
+            for (int i = 0; i < 16; i++) {
+                const int key = i / 4 * 8 + 4 * g + i % 4, j = key - mask.before;
+                const uint32_t bit = row[j < 0 ? 0 : j < a.W ? j : a.W - 1];
+                bits |= (j >= 0 && j < a.W ? bit : 0) << key;
+            }
+            sees |= all_bits(bits);
+        }
+        sees = mask.token >= 0 ? sees & mask.exists : 0;
+        const uint32_t mine = sees >> 4 * g;
+        #pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (!(mine >> (i / 4 * 8 + i % 4) & 1)) sc[i] = kNone;
+    }
+    const float mc = sums.admit(sc, a.c);
+    v8bf p[2];
+    float e[16];
+    #pragma unroll
+    for (int i = 0; i < 16; i++) {
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -mc));
+        sums.l += e[i];
+        // (what is not seen may have any scale)
+        if constexpr (FP8) e[i] = MASKED && e[i] == 0.0f ? 0.0f : e[i] * vs[i];
+    }
+    #pragma unroll
+    for (int k = 0; k < 2; k++)
+        p[k] = __builtin_bit_cast(v8bf, v4u{bf16_pack(e[8 * k], e[8 * k + 1]), bf16_pack(e[8 * k + 2], e[8 * k + 3]),
+                                            bf16_pack(e[8 * k + 4], e[8 * k + 5]), bf16_pack(e[8 * k + 6], e[8 * k + 7])});
+    // A value that is infinite or NaN reaches the rows that see its slot, and by the
+    // matrix product it would reach the others as well (0 times it is NaN): it is left out
+    // there, and added below.
+    uint64_t odd = 0;
+    if constexpr (MASKED) {
+        uint32_t most = 0;
+        #pragma unroll
+        for (int n = 0; n < D / 32; n++)
+            #pragma unroll
+            for (int k = 0; k < 2; k++)
                 #pragma unroll
-                for (int i = 1; i < 16; i++) top = fmaxf(top, sc[t][i]);
-                top = larger(top);
-                if (__builtin_amdgcn_ballot_w64(top > m[t])) {
-                    const float next = fmaxf(m[t], top);
-                    const float by = next == kNone ? 0.0f : __builtin_amdgcn_exp2f((m[t] - next) * a.c);
-                    m[t] = next;
-                    l[t] *= by;
-                    #pragma unroll
-                    for (int n = 0; n < D / 32; n++)
-                        #pragma unroll
-                        for (int c = 0; c < 16; c++) acc[t][n][c] *= by;
-                }
-                const float mc = m[t] == kNone ? 0.0f : m[t] * a.c;
-                float e[16];
-                #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], a.c, -mc));
-                    l[t] += e[i];
-                    // (what is not seen may have any scale)
-                    if constexpr (FP8) e[i] = masked && e[i] == 0.0f ? 0.0f : e[i] * vs[i];
-                }
+                for (int w = 0; w < (FP8 ? 2 : 4); w++) most = Odd<FP8>::join(most, vr[n][k][w]);
+        odd = __builtin_amdgcn_ballot_w64(Odd<FP8>::any(most));
+        if (odd) {
+            #pragma unroll
+            for (int n = 0; n < D / 32; n++)
                 #pragma unroll
                 for (int k = 0; k < 2; k++)
-                    p[t][k] = __builtin_bit_cast(v8bf, v4u{bf16_pack(e[8 * k], e[8 * k + 1]),
-                                                          bf16_pack(e[8 * k + 2], e[8 * k + 3]),
-                                                          bf16_pack(e[8 * k + 4], e[8 * k + 5]),
-                                                          bf16_pack(e[8 * k + 6], e[8 * k + 7])});
-            }
-            // A value that is infinite or NaN reaches the rows that see its slot, and by the
-            // matrix product it would reach the others as well (0 times it is NaN): it is
-            // left out there, and added below.
-            uint64_t odd = 0;
-            if constexpr (masked) {
-                uint32_t most = 0;
+                    #pragma unroll
+                    for (int w = 0; w < (FP8 ? 2 : 4); w++) vr[n][k][w] = Odd<FP8>::drop(vr[n][k][w]);
+        }
+    }
+    #pragma unroll
+    for (int n = 0; n < D / 32; n++)
+        #pragma unroll
+        for (int k = 0; k < 2; k++)
+            sums.acc[n] = mfma(FP8 ? from_fp8(vr[n][k][0], vr[n][k][1]) : __builtin_bit_cast(v8bf, vr[n][k]), p[k], sums.acc[n]);
+    if constexpr (MASKED) {
+        if (odd) {
+            for (uint32_t key = 0; key < kUnit; key++) {
+                const Lds row = stage + T::bytes + key * T::RB + g * (FP8 ? 4 : 8);
+                const uint32_t by = T::key_of_v(key);
                 #pragma unroll
-                for (int n = 0; n < D / 32; n++)
-                    #pragma unroll
-                    for (int k = 0; k < 2; k++)
+                for (int i = 0; i < D / 8; i++) {   // 4 dimensions of 8
+                    float x[4];
+                    if constexpr (FP8) {
+                        const uint32_t u = lds_read<uint32_t>(row + ((i / 2) ^ by) * 16 + i % 2 * 8);
                         #pragma unroll
-                        for (int w = 0; w < (FP8 ? 2 : 4); w++) most = Odd<FP8>::join(most, vr[n][k][w / 2][w % 2]);
-                odd = __builtin_amdgcn_ballot_w64(Odd<FP8>::any(most));
-                if (odd) {
-                    #pragma unroll
-                    for (int n = 0; n < D / 32; n++)
+                        for (int c = 0; c < 4; c++)   // (the bytes 7F and FF are NaN)
+                            x[c] = (u >> 8 * c & 0x7F) == 0x7F ? __builtin_nanf("") : 0.0f;
+                    } else {
+                        const v2u u = lds_read<v2u>(row + (i ^ by) * 16);
                         #pragma unroll
-                        for (int k = 0; k < 2; k++)
-                            #pragma unroll
-                            for (int w = 0; w < (FP8 ? 2 : 4); w++) vr[n][k][w / 2][w % 2] = Odd<FP8>::drop(vr[n][k][w / 2][w % 2]);
-                }
-            }
-            #pragma unroll
-            for (int n = 0; n < D / 32; n++) {
-                #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const v2u* x = vr[n][k];
-                    const v8bf vf = FP8 ? from_fp8(x[0][0], x[0][1])
-                                  : __builtin_bit_cast(v8bf, v4u{x[0][0], x[0][1], x[FP8 ? 0 : 1][0], x[FP8 ? 0 : 1][1]});
-                    #pragma unroll
-                    for (int t = 0; t < RT; t++) acc[t][n] = mfma(vf, p[t][k], acc[t][n]);
-                }
-            }
-            if constexpr (masked) {
-                if (odd) {
-                    for (uint32_t key = 0; key < kUnit; key++) {
-                        const uint8_t* row = stage + mine + T::bytes + key * T::RB + g * (FP8 ? 4 : 8);
-                        const uint32_t by = T::key_of_v(key);
-                        #pragma unroll
-                        for (int i = 0; i < D / 8; i++) {   // 4 dimensions of 8
-                            float x[4];
-                            if constexpr (FP8) {
-                                const uint32_t u = *reinterpret_cast<const uint32_t*>(row + ((i / 2) ^ by) * 16 + i % 2 * 8);
-                                #pragma unroll
-                                for (int c = 0; c < 4; c++)   // (the bytes 7F and FF are NaN)
-                                    x[c] = (u >> 8 * c & 0x7F) == 0x7F ? __builtin_nanf("") : 0.0f;
-                            } else {
-                                const v2u u = *reinterpret_cast<const v2u*>(row + (i ^ by) * 16);
-                                #pragma unroll
-                                for (int c = 0; c < 4; c++) {
-                                    x[c] = c % 2 ? bf16_hi(u[c / 2]) : bf16_lo(u[c / 2]);
-                                    if (__builtin_isfinite(x[c])) x[c] = 0.0f;
-                                }
-                            }
-                            #pragma unroll
-                            for (int t = 0; t < RT; t++)
-                                if (sees[t] >> key & 1)
-                                    #pragma unroll
-                                    for (int c = 0; c < 4; c++) acc[t][i / 4][i % 4 * 4 + c] += x[c];
+                        for (int c = 0; c < 4; c++) {
+                            x[c] = c % 2 ? bf16_hi(u[c / 2]) : bf16_lo(u[c / 2]);
+                            if (__builtin_isfinite(x[c])) x[c] = 0.0f;
                         }
                     }
+                    if (sees >> key & 1)
+                        #pragma unroll
+                        for (int c = 0; c < 4; c++) sums.acc[i / 4][i % 4 * 4 + c] += x[c];
                 }
+            }
+        }
+    }
+}
+
+// A workgroup's run of the work, item by item.
+struct Item {
+    int h, tile, first, end;   // row tile `tile` of cache head h, units first .. end - 1 of it
+    bool whole;                // all of its units
+    bool cut;                  // it began in another workgroup's run
+};
+struct Run {
+    int64_t left, in;   // pieces; the next one's number in its sequence
+    int b;
+    Seq s;
+    __device__ __forceinline__ bool begin(const Args& a) {
+        int64_t all, none;
+        total_cost(a, 0, all, none);
+        const int groups = a.work.whole ? 0 : work_groups(a.work, all);
+        if (a.work.whole ? (int64_t)blockIdx.x >= all : (int)blockIdx.x >= groups) return false;
+        in = a.work.whole ? (int64_t)blockIdx.x : range_start(all, groups, blockIdx.x);
+        left = a.work.whole ? 1 : range_start(all, groups, blockIdx.x + 1) - in;
+        b = find_piece(a, in);
+        s = sequence(a, b);
+        return true;
+    }
+    __device__ __forceinline__ Item take(const Args& a) {
+        Item o;
+        if (a.work.whole) {
+            o.h = (int)(in % a.batch.heads);
+            o.tile = s.tiles - 1 - (int)(in / a.batch.heads);
+            o.first = 0;
+            o.end = s.units;
+            o.whole = true;
+            o.cut = false;
+            left = 0;
+            return o;
+        }
+        const int pieces = s.units + a.work.item;
+        const int64_t item = in / pieces;
+        const int from = (int)(in - item * pieces);
+        o.h = (int)(item / s.tiles);
+        o.tile = (int)(item - (int64_t)o.h * s.tiles);
+        const int to = (int)(from + left < pieces ? from + left : pieces);
+        o.first = max(0, from - a.work.item);
+        o.end = to - a.work.item;   // (none of its units if not above first)
+        o.whole = o.first == 0 && o.end == s.units;
+        o.cut = o.first > 0;
+        left -= to - from;
+        in += to - from;
+        return o;
+    }
+    // The next item's sequence; false if there is none.
+    __device__ __forceinline__ bool go_on(const Args& a) {
+        if (left <= 0) return false;
+        if (in == (int64_t)a.batch.heads * s.tiles * (s.units + a.work.item)) {
+            in = 0;
+            do {
+                if (++b == a.batch.B) return false;   // (not reached while nobody writes to the batch)
+                s = sequence(a, b);
+            } while (s.tiles == 0);
+        }
+        return true;
+    }
+    // The units of an item that are computed end here: without a mask no row of the tile
+    // sees a slot past its last token's.
+    __device__ __forceinline__ int stop(const Args& a, const Item& o, int rows) const {
+        if (a.mask) return o.end;
+        const int last = min(s.tokens - 1, (o.tile * rows + rows - 1) / a.G);
+        return min(o.end, slot_units((int)min((int64_t)s.slots, (int64_t)s.context + last + 1)));
+    }
+    // Below it every row of the tile sees all of a unit's slots, if they exist.
+    __device__ __forceinline__ int plain(const Args& a, const Item& o, int rows, int stop) const {
+        return min(stop, (int)(((int64_t)s.context + (a.mask ? 0 : o.tile * rows / a.G + 1)) / kUnit));
+    }
+};
+
+// The rows of a unit of the item's slots, looked up in the table well before they are
+// loaded: lane (g, r) has slot r's.
+struct Lookup { uint32_t entry, off; bool in; };
+__device__ __forceinline__ Lookup look_up(const Args& a, const Run& run, int u, int stop) {
+    const uint32_t slot = (uint32_t)u * kUnit + (threadIdx.x & 31);
+    Lookup o;
+    o.in = u < stop && slot < (uint32_t)run.s.slots;
+    const uint32_t i = o.in ? a.batch.page_of(slot) : 0;
+    o.off = slot - i * a.batch.page;
+    o.entry = run.s.slots > 0 ? (uint32_t)a.batch.table[(int64_t)run.b * a.batch.per + i] : 0;
+    return o;
+}
+
+// Loads a unit's rows (of nothing: row 0's, which no lane sees) into a stage, its share
+// if the workgroup's NW waves share it; returns the slots that exist.
+template <int D, bool FP8, int NW>
+__device__ __forceinline__ uint32_t load_unit(const Args& a, const Lookup& o, int h, Lds stage, Lds scales) {
+    using T = Tile<D, FP8>;
+    constexpr int kLoads = 2 * T::loads / NW, kDistinct = NW > 1 ? kLoads : T::loads;
+    static_assert(2 * T::loads % NW == 0, "loads");
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes) : 0;
+    const bool valid = o.in && o.entry < a.batch.pages;
+    const uint32_t row = valid ? (o.entry * a.batch.heads + h) * a.batch.page + o.off : 0;
+    const uint32_t exists = (uint32_t)__builtin_amdgcn_ballot_w64(valid);
+    // K's loads, then V's; the rows that a lane loads come from their lanes
+    auto of = [&](int i) { return (wave * kLoads + i) % T::loads * T::per_load + lane / T::pieces; };
+    uint32_t from[kDistinct];
+    #pragma unroll
+    for (int i = 0; i < kDistinct; i++) from[i] = __shfl(row, of(i));
+    #pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+        const int n = wave * kLoads + i;
+        const bool is_v = n >= T::loads;
+        const uint32_t at = of(i % kDistinct), key = is_v ? T::key_of_v(at) : T::key_of_k(at);
+        load_lds<16>((is_v ? a.v : a.k) + (int64_t)from[i % kDistinct] * T::RB + ((lane % T::pieces) ^ key) * 16,
+                     stage + n * 1024);
+    }
+    if constexpr (FP8) load_lds<4>((lane >> 5 ? a.v_scale : a.k_scale) + row, scales);
+    return exists;
+}
+
+// Where an item's sums go: to `out`, or to its part.
+struct Target {
+    uint16_t* out;
+    float *part_o, *part_s;
+    bool parts;
+};
+template <int D>
+__device__ __forceinline__ Target target(const Args& a, const Run& run, const Item& o, int rows) {
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (o.cut ? 0 : 1);
+    return {a.out, a.parts + slot * rows * D,
+            a.parts + ((int64_t)a.work.groups * 2 * rows * D) + slot * rows * 2, !o.whole};
+}
+__device__ __forceinline__ int64_t out_row(const Args& a, const Run& run, const Item& o, int row) {
+    return (int64_t)(run.s.start + row / a.G) * a.Hq + o.h * a.G + row % a.G;
+}
+
+// Few rows: every wave takes all 32 RT rows of the tile and every NW-th unit, through a
+// ring of its own in LDS that loads write without a register between; the waves' sums are
+// added at the end.  Nothing makes the waves wait for each other, so that each keeps its
+// ring's loads under way.
+template <int D, bool FP8, int RT, int NW, int STAGES>
+__global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
+    using T = Tile<D, FP8>;
+    constexpr int kRows = 32 * RT;
+    constexpr int kIssue = 2 * T::loads + (FP8 ? 1 : 0);   // a unit's loads, with the scales'
+    constexpr int kStage = 2 * T::bytes + (FP8 ? 256 : 0);
+    constexpr int kRing = kStage * NW;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring0[kRing], ring1[kRing],
+        ring2[STAGES > 2 ? kRing : 16], ring3[STAGES > 3 ? kRing : 16];
+    __shared__ float stat[NW][kRows][2];
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int r = lane & 31, g = lane >> 5;
+    const uint32_t mine = wave * kStage;
+    Run run;
+    if (!run.begin(a)) return;
+    Places<D, FP8> at;
+    at.set(lane);
+
+    do {
+        const Item o = run.take(a);
+        if (o.end <= o.first) continue;
+        const Seq& s = run.s;
+        const int rows = s.tokens * a.G, stop = run.stop(a, o, kRows), plain = run.plain(a, o, kRows, stop);
+        v8bf q[RT][D / 16];
+        Mask mask[RT];
+        Sums<D> sums[RT];
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int row = o.tile * kRows + 32 * t + r;
+            mask[t].token = row < rows ? row / a.G : -1;
+            mask[t].start = s.start;
+            load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask[t].token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
+                               row < rows, q[t]);
+            sums[t].clear();
+        }
+        auto compute = [&](auto MASKED, int u, uint32_t exists, Lds stage) {
+            #pragma unroll
+            for (int t = 0; t < RT; t++) {
+                mask[t].before = s.context - u * kUnit;
+                mask[t].exists = exists;
+                attend_unit<D, FP8, decltype(MASKED)::value>(a, at, stage + mine, stage + mine + 2 * T::bytes, q[t], sums[t], mask[t]);
+                // (the second tile reads the stage again: its operands in registers from one
+                // tile to the next would be more than there are)
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" ::: "memory");
             }
         };
 
-
-        // A wave's units: every one, or the NW-th from its own on.  Below `plain` every row
-        // sees all of a unit's slots, if they exist.
-        constexpr int kBy = SHARED ? 1 : NW;
-        const int plain = min(stop, (int)(((int64_t)s.context + (a.mask ? 0 : tile * kRows / a.G + 1)) / kUnit));
-        const int u0 = first + (SHARED ? 0 : wave);
-        uint8_t* const rings[4] = {ring0, ring1, ring2, ring3};
+        const Lds rings[4] = {(Lds)ring0, (Lds)ring1, (Lds)ring2, (Lds)ring3};
         uint32_t exists[STAGES];
         Lookup la, lb;
         auto fetch = [&](int v, int i) {   // unit v, whose lookup is la, into stage i
             const Lookup l = la;
             la = lb;
-            lb = look_up(v + 2 * kBy);
-            exists[i] = issue(l, rings[i]);
+            lb = look_up(a, run, v + 2 * NW, stop);
+            exists[i] = load_unit<D, FP8, 1>(a, l, o.h, rings[i] + mine, rings[i] + mine + 2 * T::bytes);
         };
-        constexpr int kAhead = SHARED ? STAGES - 1 : STAGES;   // units under way
         auto begin = [&](int v) {
-            la = look_up(v);
-            lb = look_up(v + kBy);
+            la = look_up(a, run, v, stop);
+            lb = look_up(a, run, v + NW, stop);
             #pragma unroll
-            for (int i = 0; i < kAhead; i++) fetch(v + i * kBy, i);
+            for (int i = 0; i < STAGES; i++) fetch(v + i * NW, i);
         };
+        const int u0 = o.first + wave;
+        int u = u0;
         begin(u0);
         // Plain units, a round of the stages at a time (an exit between two stages would
         // make the compiler wait for all loads in each).
-        int u = u0;
         uint32_t whole = 0xFFFFFFFFu;
-        while (u + (STAGES - 1) * kBy < plain) {
+        while (u + (STAGES - 1) * NW < plain) {
             #pragma unroll
             for (int i = 0; i < STAGES; i++) {
-                if constexpr (SHARED) {
-                    arrive<(kAhead - 1) * kIssue>();
-                    whole &= exists[i];
-                    // (the stage that all waves have read before the barrier)
-                    fetch(u + kAhead, (i + kAhead) % STAGES);
-                    compute(std::false_type{}, u, 0, rings[i]);
-                } else {
-                    wait_loads<(kAhead - 1) * kIssue>();
-                    whole &= exists[i];
-                    compute(std::false_type{}, u, 0, rings[i]);
-                    // (the reads of this stage have come: the products have used them)
-                    __builtin_amdgcn_sched_barrier(0);
-                    asm volatile("" ::: "memory");
-                    fetch(u + STAGES * kBy, i);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                u += kBy;
+                wait_loads<(STAGES - 1) * kIssue>();
+                whole &= exists[i];
+                compute(std::false_type{}, u, 0, rings[i]);
+                // (the reads of this stage have come: the products have used them)
+                fetch(u + STAGES * NW, i);
+                __builtin_amdgcn_sched_barrier(0);
+                u += NW;
             }
         }
         if (__builtin_amdgcn_readfirstlane(whole) != 0xFFFFFFFFu) {
             // some of them were of pages that do not exist: all over again, slot by slot
-            if constexpr (SHARED) arrive<0>(); else wait_loads<0>();
-            clear();
+            wait_loads<0>();
+            #pragma unroll
+            for (int t = 0; t < RT; t++) sums[t].clear();
             u = u0;
             begin(u);
         }
-        // The others: kAhead units lie in the stages from the first on.
+        // The others: they lie in the stages from the first on.
         while (true) {
-            if constexpr (SHARED) arrive<0>(); else wait_loads<0>();
-            for (int i = 0; i < kAhead && u < stop; i++, u += kBy) {
-                const uint8_t* stage = i == 0 ? ring0 : i == 1 ? ring1 : i == 2 ? ring2 : ring3;
+            wait_loads<0>();
+            for (int i = 0; i < STAGES && u < stop; i++, u += NW) {
+                const Lds stage = i == 0 ? rings[0] : i == 1 ? rings[1] : i == 2 ? rings[2] : rings[3];
                 uint32_t e = exists[0];
                 #pragma unroll
-                for (int k = 1; k < kAhead; k++) e = i == k ? exists[k] : e;
+                for (int k = 1; k < STAGES; k++) e = i == k ? exists[k] : e;
                 compute(std::true_type{}, u, e, stage);
             }
             if (u >= stop) break;
-            if constexpr (SHARED) arrive<0>();
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("" ::: "memory");
             #pragma unroll
-            for (int i = 0; i < kAhead; i++) fetch(u + i * kBy, i);
+            for (int i = 0; i < STAGES; i++) fetch(u + i * NW, i);
         }
-        if constexpr (SHARED) arrive<0>();   // (before the ring is filled again)
 
+        // The waves' sums are added in wave order, brought to the largest of their maxima.
+        const Target to = target<D>(a, run, o, kRows);
         #pragma unroll
-        for (int t = 0; t < RT; t++) l[t] = sum_of(l[t]);
-        const bool to_parts = !is_whole;
-        const int64_t slot = (int64_t)blockIdx.x * 2 + (cut ? 0 : 1);
-        float* part_o = a.parts + slot * kRows * D;
-        float* part_s = a.parts + ((int64_t)a.work.groups * 2 * kRows * D) + slot * kRows * 2;
-        auto out_row = [&](int row) {   // of q's rows, out
-            return a.out + ((int64_t)(s.start + row / a.G) * a.Hq + h * a.G + row % a.G) * D;
+        for (int t = 0; t < RT; t++) {
+            sums[t].l = sum_of(sums[t].l);
+            if (g == 0) {
+                stat[wave][32 * t + r][0] = sums[t].m;
+                stat[wave][32 * t + r][1] = sums[t].l;
+            }
+        }
+        __syncthreads();   // (all waves' loads into the ring have come, and their reads)
+        constexpr int kHold = 32 * RT * D * 4;   // bytes of a wave's sums
+        auto held = [&](int w) {   // (rings of whole waves' sums)
+            constexpr int kPer = kRing / kHold;
+            static_assert(kPer >= 1 && kPer * STAGES >= NW, "the rings hold the sums");
+            const int i = w / kPer;
+            return (i == 0 ? rings[0] : i == 1 ? rings[1] : i == 2 ? rings[2] : rings[3]) + w % kPer * kHold;
         };
-        if constexpr (SHARED) {
+        const Lds hold = held(wave);
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float top = kNone;
             #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const int row = row0 + 32 * t + r, local = row - tile * kRows;
-                if (row >= rows) continue;
-                const float by = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
-                if (to_parts && g == 0) {
-                    part_s[local * 2] = m[t];
-                    part_s[local * 2 + 1] = l[t];
-                }
-                uint16_t* o = out_row(row);
+            for (int w = 0; w < NW; w++) top = fmaxf(top, stat[w][32 * t + r][0]);
+            const float by = sums[t].m == kNone ? 0.0f : __builtin_amdgcn_exp2f((sums[t].m - top) * a.c);
+            #pragma unroll
+            for (int n = 0; n < D / 32; n++)
                 #pragma unroll
-                for (int n = 0; n < D / 32; n++)
+                for (int i = 0; i < 4; i++) {
+                    const int row = 32 * t + r, piece = 8 * n + 2 * i + g;
+                    const v16f& x = sums[t].acc[n];
+                    *(TANS_LDS v4f*)(hold + row * D * 4 + (piece ^ (row & 15)) * 16) =
+                        v4f{x[4 * i] * by, x[4 * i + 1] * by, x[4 * i + 2] * by, x[4 * i + 3] * by};
+                }
+        }
+        __syncthreads();
+        const int valid = min(kRows, rows - o.tile * kRows);
+        for (int x = threadIdx.x; x < valid * (D / 4); x += NW * kLanes) {
+            const int row = x / (D / 4), piece = x % (D / 4);
+            float top = kNone, sum = 0.0f;
+            #pragma unroll
+            for (int w = 0; w < NW; w++) top = fmaxf(top, stat[w][row][0]);
+            v4f f = {0, 0, 0, 0};
+            #pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float mw = stat[w][row][0];
+                sum += mw == kNone ? 0.0f : stat[w][row][1] * __builtin_amdgcn_exp2f((mw - top) * a.c);
+                f += lds_read<v4f>(held(w) + row * D * 4 + (piece ^ (row & 15)) * 16);
+            }
+            if (to.parts) {
+                *reinterpret_cast<v4f*>(to.part_o + row * D + piece * 4) = f;
+                if (piece == 0) {
+                    to.part_s[row * 2] = top;
+                    to.part_s[row * 2 + 1] = sum;
+                }
+            } else {
+                const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+                *reinterpret_cast<v2u*>(to.out + out_row(a, run, o, o.tile * kRows + row) * D + piece * 4) =
+                    v2u{bf16_pack(f[0] * by, f[1] * by), bf16_pack(f[2] * by, f[3] * by)};
+            }
+        }
+        if (run.left > 0) __syncthreads();   // (before the ring is filled again)
+    } while (run.go_on(a));
+}
+
+// Many rows: each of four waves takes 32 RT rows of the tile and all units, which pass
+// through LDS once for all four.  The products of one part run beside the exponentials of
+// another, in one wave's own instructions, step by step (a step is a matrix instruction
+// and what fits beside it):
+//
+//   RT = 2   the row tiles take turns: the products of tile 0 (K's with the next unit, V's
+//            with this one) beside the exponentials of tile 1, then the other way around.
+//            Operands of K and V are read from LDS once for both.
+//   RT = 1   the next unit's products with K beside this one's exponentials, then V's.
+template <int D, bool FP8, int RT>
+__global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
+    using T = Tile<D, FP8>;
+    constexpr int NW = 4, STAGES = 4;
+    constexpr int kRows = 32 * RT * NW;
+    constexpr int kIssue = 2 * T::loads / NW + (FP8 ? 1 : 0);   // a wave's loads of a unit
+    constexpr int kStage = 2 * T::bytes + (FP8 ? 256 * NW : 0);
+    constexpr int kSteps = D / 16;   // products with K, and with V, of a unit and 32 rows
+    __shared__ __attribute__((aligned(1024))) uint8_t ring0[kStage], ring1[kStage], ring2[kStage], ring3[kStage];
+    const Lds rings[4] = {(Lds)ring0, (Lds)ring1, (Lds)ring2, (Lds)ring3};
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int r = lane & 31, g = lane >> 5;
+    const uint32_t my_scales = 2 * T::bytes + wave * 256;
+    Run run;
+    if (!run.begin(a)) return;
+    Places<D, FP8> at;
+    at.set(lane);
+
+    do {
+        const Item o = run.take(a);
+        if (o.end <= o.first) continue;
+        const Seq& s = run.s;
+        const int rows = s.tokens * a.G, row0 = o.tile * kRows + wave * 32 * RT;
+        const int stop = run.stop(a, o, kRows), plain = run.plain(a, o, kRows, stop);
+        v8bf q[RT][D / 16];
+        Mask mask[RT];
+        Sums<D> sums[RT];
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int row = row0 + 32 * t + r;
+            mask[t].token = row < rows ? row / a.G : -1;
+            mask[t].start = s.start;
+            load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask[t].token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
+                               row < rows, q[t]);
+            sums[t].clear();
+        }
+        uint32_t exists[STAGES];
+        Lookup la, lb;
+        auto fetch = [&](int v, int i) {   // unit v, whose lookup is la, into stage i
+            const Lookup l = la;
+            la = lb;
+            lb = look_up(a, run, v + 2, stop);
+            exists[i] = load_unit<D, FP8, NW>(a, l, o.h, rings[i], rings[i] + my_scales);
+        };
+        auto begin = [&](int v) {
+            la = look_up(a, run, v, stop);
+            lb = look_up(a, run, v + 1, stop);
+            #pragma unroll
+            for (int i = 0; i < STAGES; i++) fetch(v + i, i);
+        };
+        int u = o.first;
+        if (u < stop) begin(u);
+
+        // Plain units: the first, and then rounds of the stages.
+        uint32_t whole = 0xFFFFFFFFu;
+        const int rounds = plain > u ? (plain - u - 1) / STAGES : 0;
+        if (plain > u) {
+            v16f sc[2];
+            v4u kr[kSteps], vr[kSteps];       // operands as they were read
+            v8bf kf[kSteps], vf[kSteps];      // and as the products take them
+            float ks[FP8 ? 16 : 1], vs[FP8 ? 16 : 1], e[16], mc = 0.0f;
+            uint32_t p[RT][8];
+            auto read_k = [&](Lds stage, int j) {
+                if (!FP8 || j % 2 == 0) kr[j] = at.read_k(stage, j);
+            };
+            auto read_v = [&](Lds stage, int x) { vr[x] = at.read_v(stage, x % (D / 32), x / (D / 32)); };
+            auto take_k = [&](int j) {
+                const v4u& x = kr[FP8 ? j / 2 * 2 : j];
+                kf[j] = FP8 ? from_fp8(x[2 * (j % 2)], x[2 * (j % 2) + 1]) : __builtin_bit_cast(v8bf, x);
+            };
+            auto take_v = [&](int x) { vf[x] = FP8 ? from_fp8(vr[x][0], vr[x][1]) : __builtin_bit_cast(v8bf, vr[x]); };
+            auto with_k = [&](v16f& to, int t, int j) {
+                v16f zero = {};
+                to = mfma(kf[j], q[t][j], j == 0 ? zero : to);
+            };
+            auto with_v = [&](int t, int x) {
+                const uint32_t* w = p[t] + x / (D / 32) * 4;
+                sums[t].acc[x % (D / 32)] = mfma(vf[x], __builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]}),
+                                                 sums[t].acc[x % (D / 32)]);
+            };
+            auto step = [] {
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" ::: "memory");
+            };
+            // Softmax of tile t's scores, in steps 0 .. n - 1.
+            auto softmax = [&](v16f& x, int t, int i, int n) {
+                if (i == 0) {
+                    if constexpr (FP8)
+                        #pragma unroll
+                        for (int c = 0; c < 16; c++) x[c] *= ks[c];
+                    mc = sums[t].admit(x, a.c);
+                } else {
                     #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int d = 32 * n + 8 * i + 4 * g;
-                        const v4f x = {acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]};
-                        if (to_parts) {
-                            *reinterpret_cast<v4f*>(part_o + local * D + d) = x;
-                        } else {
-                            *reinterpret_cast<v2u*>(o + d) = v2u{bf16_pack(x[0] * by, x[1] * by), bf16_pack(x[2] * by, x[3] * by)};
+                    for (int c = 16 * (i - 1) / (n - 1); c < 16 * i / (n - 1); c++) {
+                        e[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c], a.c, -mc));
+                        sums[t].l += e[c];
+                        if constexpr (FP8) e[c] *= vs[c];
+                        if (c % 2) p[t][c / 2] = bf16_pack(e[c - 1], e[c]);
+                    }
+                }
+            };
+            auto scales = [&](Lds stage) {
+                if constexpr (FP8) {
+                    read_scales(stage + my_scales, ks);
+                    read_scales(stage + my_scales + 128, vs);
+                }
+            };
+
+            arrive<2 * kIssue>();   // the first two units
+            #pragma unroll
+            for (int j = 0; j < kSteps; j++) read_k(rings[0], j);
+            scales(rings[0]);
+            #pragma unroll
+            for (int j = 0; j < kSteps; j++) {
+                take_k(j);
+                with_k(sc[0], 0, j);
+                if constexpr (RT == 2) with_k(sc[1], 1, j);
+            }
+            whole &= exists[0];
+            #pragma unroll
+            for (int j = 0; j < kSteps; j++) {
+                read_k(rings[1], j);
+                if constexpr (RT == 2) read_v(rings[0], j);
+            }
+            if constexpr (RT == 2) {
+                #pragma unroll
+                for (int i = 0; i < 2 * kSteps; i++) softmax(sc[0], 0, i, 2 * kSteps);
+            }
+            for (int n = 0; n < rounds; n++) {
+                #pragma unroll
+                for (int i = 0; i < STAGES; i++) {   // unit u, in stage i
+                    const Lds st1 = rings[(i + 1) % STAGES], st2 = rings[(i + 2) % STAGES];
+                    if constexpr (RT == 2) {
+                        #pragma unroll
+                        for (int j = 0; j < 2 * kSteps; j++) {
+                            if (j < kSteps) {
+                                take_k(j);
+                                with_k(sc[0], 0, j);
+                            } else {
+                                take_v(j - kSteps);
+                                with_v(0, j - kSteps);
+                            }
+                            softmax(sc[1], 1, j, 2 * kSteps);
+                            step();
+                        }
+                        whole &= exists[(i + 1) % STAGES];
+                        arrive<kIssue>();   // unit u + 2; unit u has been read
+                        scales(st1);
+                        fetch(u + STAGES, i);
+                        #pragma unroll
+                        for (int j = 0; j < 2 * kSteps; j++) {
+                            if (j < kSteps) {
+                                with_k(sc[1], 1, j);
+                                softmax(sc[0], 0, j, 2 * kSteps);
+                                read_k(st2, j);
+                            } else {
+                                with_v(1, j - kSteps);
+                                softmax(sc[0], 0, j, 2 * kSteps);
+                                read_v(st1, j - kSteps);
+                            }
+                            step();
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int j = 0; j < kSteps; j++) {
+                            take_k(j);
+                            with_k(sc[(i + 1) % 2], 0, j);
+                            softmax(sc[i % 2], 0, j, kSteps);
+                            if (2 * j < kSteps) {
+                                read_v(rings[i], 2 * j);
+                                read_v(rings[i], 2 * j + 1);
+                            }
+                            step();
+                        }
+                        whole &= exists[(i + 1) % STAGES];
+                        arrive<kIssue>();   // unit u + 2; unit u has been read
+                        fetch(u + STAGES, i);
+                        #pragma unroll
+                        for (int j = 0; j < kSteps; j++) {
+                            take_v(j);
+                            with_v(0, j);
+                            read_k(st2, j);
+                            if (j == 0) scales(st1);
+                            step();
                         }
                     }
+                    u++;
+                }
             }
-        } else {
-            // The waves' sums are added in wave order, brought to the largest of their maxima.
+            // the last one's rest
+            if constexpr (RT == 1) {
+                #pragma unroll
+                for (int x = 0; x < kSteps; x++) read_v(rings[0], x);
+            }
             #pragma unroll
-            for (int t = 0; t < RT; t++)
-                if (g == 0) {
-                    stat[wave][32 * t + r][0] = m[t];
-                    stat[wave][32 * t + r][1] = l[t];
-                }
-            __syncthreads();   // (all waves' loads into the ring have come, and their reads)
-            constexpr int kHold = 32 * RT * D * 4;   // bytes of a wave's sums
-            auto held = [&](int w) {   // (rings of whole waves' sums)
-                constexpr int kPer = kRing / kHold;
-                static_assert(kPer >= 1 && kPer * STAGES >= NW, "the rings hold the sums");
-                uint8_t* ring = w / kPer == 0 ? ring0 : w / kPer == 1 ? ring1 : w / kPer == 2 ? ring2 : ring3;
-                return (float*)(ring + w % kPer * kHold);
-            };
-            float* hold = held(wave);
+            for (int i = 0; i < 2 * kSteps; i++) softmax(sc[RT - 1], RT - 1, i, 2 * kSteps);
             #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                float top = kNone;
+            for (int x = 0; x < kSteps; x++) {
+                take_v(x);
                 #pragma unroll
-                for (int w = 0; w < NW; w++) top = fmaxf(top, stat[w][32 * t + r][0]);
-                const float by = m[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f((m[t] - top) * a.c);
-                #pragma unroll
-                for (int n = 0; n < D / 32; n++)
-                    #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int row = 32 * t + r, piece = 8 * n + 2 * i + g;
-                        *reinterpret_cast<v4f*>(hold + row * D + (piece ^ (row & 15)) * 4) =
-                            v4f{acc[t][n][4 * i] * by, acc[t][n][4 * i + 1] * by, acc[t][n][4 * i + 2] * by,
-                                acc[t][n][4 * i + 3] * by};
-                    }
+                for (int t = 0; t < RT; t++) with_v(t, x);
             }
-            __syncthreads();
-            const int valid = min(kRows, rows - tile * kRows);
-            for (int x = threadIdx.x; x < valid * (D / 4); x += NW * kLanes) {
-                const int row = x / (D / 4), piece = x % (D / 4);
-                float top = kNone, sum = 0.0f;
+            u++;
+            arrive<0>();   // (before the ring is filled again)
+            if (__builtin_amdgcn_readfirstlane(whole) != 0xFFFFFFFFu) {
+                // some of them were of pages that do not exist: all over again, slot by slot
                 #pragma unroll
-                for (int w = 0; w < NW; w++) top = fmaxf(top, stat[w][row][0]);
-                v4f o = {0, 0, 0, 0};
+                for (int t = 0; t < RT; t++) sums[t].clear();
+                u = o.first;
+            }
+            if (u < stop) begin(u);
+        }
+        // The others: they lie in the stages from the first on.
+        while (u < stop) {
+            arrive<0>();
+            for (int i = 0; i < STAGES && u < stop; i++, u++) {
+                const Lds stage = i == 0 ? rings[0] : i == 1 ? rings[1] : i == 2 ? rings[2] : rings[3];
+                uint32_t e = exists[0];
                 #pragma unroll
-                for (int w = 0; w < NW; w++) {
-                    const float mw = stat[w][row][0];
-                    sum += mw == kNone ? 0.0f : stat[w][row][1] * __builtin_amdgcn_exp2f((mw - top) * a.c);
-                    o += *reinterpret_cast<const v4f*>(held(w) + row * D + (piece ^ (row & 15)) * 4);
-                }
-                if (to_parts) {
-                    *reinterpret_cast<v4f*>(part_o + row * D + piece * 4) = o;
-                    if (piece == 0) {
-                        part_s[row * 2] = top;
-                        part_s[row * 2 + 1] = sum;
-                    }
-                } else {
-                    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    *reinterpret_cast<v2u*>(out_row(tile * kRows + row) + piece * 4) =
-                        v2u{bf16_pack(o[0] * by, o[1] * by), bf16_pack(o[2] * by, o[3] * by)};
+                for (int k = 1; k < STAGES; k++) e = i == k ? exists[k] : e;
+                #pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    mask[t].before = s.context - u * kUnit;
+                    mask[t].exists = e;
+                    attend_unit<D, FP8, true>(a, at, stage, stage + my_scales, q[t], sums[t], mask[t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" ::: "memory");
                 }
             }
-            if (left > 0) __syncthreads();   // (before the ring is filled again)
+            arrive<0>();   // (before the ring is filled again)
+            if (u < stop) {
+                #pragma unroll
+                for (int i = 0; i < STAGES; i++) fetch(u + i, i);
+            }
         }
+
+        const Target to = target<D>(a, run, o, kRows);
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const float l = sum_of(sums[t].l);
+            const int row = row0 + 32 * t + r, local = row - o.tile * kRows;
+            if (row >= rows) continue;
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
+            if (to.parts && g == 0) {
+                to.part_s[local * 2] = sums[t].m;
+                to.part_s[local * 2 + 1] = l;
+            }
+            uint16_t* out = to.out + out_row(a, run, o, row) * D;
+            #pragma unroll
+            for (int n = 0; n < D / 32; n++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int d = 32 * n + 8 * i + 4 * g;
+                    const v16f& c = sums[t].acc[n];
+                    const v4f x = {c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]};
+                    if (to.parts)
+                        *reinterpret_cast<v4f*>(to.part_o + local * D + d) = x;
+                    else
+                        *reinterpret_cast<v2u*>(out + d) = v2u{bf16_pack(x[0] * by, x[1] * by), bf16_pack(x[2] * by, x[3] * by)};
+                }
         }
-        // the next item's sequence
-        if (left > 0 && in == (int64_t)a.batch.heads * s.tiles * (s.units + a.work.item)) {
-            in = 0;
-            do {
-                if (++b == a.batch.B) return;   // (not reached while nobody writes to the batch)
-                s = sequence(a, b);
-            } while (s.tiles == 0);
-        }
-    }
+    } while (run.go_on(a));
 }
 
 // The rows of items that several workgroups share, from their parts in the order of
@@ -835,7 +1147,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         return fail(TANS_EINVAL, op + ": workspace too small, null or misaligned (16 bytes)");
     if (p.blocks > INT32_MAX / 256) return fail(TANS_EINVAL, op + ": too many tokens for one call");
     Args a = {};
-    a.batch = {table, starts, lens, (int)B, (int)per, (int)N, (uint32_t)pages, (uint32_t)heads, (uint32_t)page};
+    a.batch = make_batch(table, starts, lens, B, per, N, pages, heads, page);
     a.q = (const uint16_t*)q;
     a.q_stride = q_stride;
     a.k = (const uint8_t*)k_cache;
@@ -861,12 +1173,12 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         constexpr int stage = (2 * Tile<D, f8>::bytes + (f8 ? 256 : 0)) * nw;
         constexpr int stages = 4 * stage <= (132 << 10) ? 4 : 2;
         int rc;
-        if (p.kind == kFew) rc = launch(attend_kernel<D, f8, 1, false, nw, stages>, nw * kLanes);
-        else if (p.kind == kMany) rc = launch(attend_kernel<D, f8, 1, true, 4, 3>, 4 * kLanes);
+        if (p.kind == kFew) rc = launch(attend_kernel<D, f8, 1, nw, stages>, nw * kLanes);
+        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 1>, 4 * kLanes);
         else {
             if constexpr (D < 256) {
-                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, false, nw, stages>, nw * kLanes);
-                else rc = launch(attend_kernel<D, f8, 2, true, 4, 3>, 4 * kLanes);
+                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages>, nw * kLanes);
+                else rc = launch(attend_rows_kernel<D, f8, 2>, 4 * kLanes);
             } else {
                 rc = fail(TANS_EINVAL, "tree_attention: no such kernel");   // (not reached: plan())
             }

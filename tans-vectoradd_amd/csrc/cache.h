@@ -25,6 +25,21 @@ __device__ __forceinline__ int find_sequence(const Batch& batch, int n) {
 
 // Host side ---------------------------------------------------------------
 
+inline Batch make_batch(const int32_t* table, const int32_t* starts, const int32_t* lens, int64_t B,
+                        int64_t per, int64_t N, int64_t pages, int64_t heads, int64_t page) {
+    Batch b = {};
+    b.table = table;
+    b.starts = starts;
+    b.lens = lens;
+    b.B = (int)B;
+    b.per = (int)per;
+    b.N = (int)N;
+    b.pages = (uint32_t)pages;
+    b.heads = (uint32_t)heads;
+    b.set_page((uint32_t)page);
+    return b;
+}
+
 // The batch's sizes and pointers, alike for both operators.
 inline int batch_check(const std::string& op, const void* k, const void* v, const void* k_scale,
                        const void* v_scale, int64_t pages, int64_t heads, int64_t page, int64_t dim,

@@ -30,7 +30,21 @@ struct Batch {
     const int32_t* lens;     // [B]
     int B, per, N;           // N: rows of q
     uint32_t pages, heads, page;
+    // slot / page = (slot * inverse) >> (31 + shift) for slots below 2^31: inverse is 2^(31 +
+    // shift) / page rounded up, with 2^shift >= page, so it is too large by less than 1, and the
+    // quotient by less than 2^31 / 2^(31 + shift) <= 1 / page
+    uint32_t inverse;
+    int shift;
 
+    inline void set_page(uint32_t rows) {
+        page = rows;
+        shift = 0;
+        while ((uint32_t(1) << shift) < rows) shift++;
+        inverse = (uint32_t)(((uint64_t(1) << (31 + shift)) + rows - 1) / rows);
+    }
+    TANS_BOTH uint32_t page_of(uint32_t slot) const {
+        return (uint32_t)((uint64_t)(2 * slot) * inverse >> 32) >> shift;
+    }
     TANS_BOTH int64_t capacity() const { return (int64_t)per * page; }
     TANS_BOTH int start(int b) const {
         const int s = starts[b];
@@ -48,7 +62,7 @@ struct Batch {
     // Row of the cache (of all heads' and pages') of slot s < capacity() and head h;
     // false if the table's entry is no page.
     TANS_BOTH bool row(int b, uint32_t s, uint32_t h, uint32_t& r) const {
-        const uint32_t i = s / page, p = (uint32_t)table[(int64_t)b * per + i];
+        const uint32_t i = page_of(s), p = (uint32_t)table[(int64_t)b * per + i];
         r = (p * heads + h) * page + (s - i * page);
         return p < pages;
     }

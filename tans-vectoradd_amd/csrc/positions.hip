@@ -291,8 +291,7 @@ int tans_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k
     const int tokens = kThreads / kLanes / waves;
     if ((N + tokens - 1) / tokens > (1 << 23)) return fail(TANS_EINVAL, op + ": too many tokens for one call");
     const Rotation r = {positions, frequencies, (int)rot, (int)dim, magnitude, 1.0f};
-    const Batch batch = {table, starts, lens, (int)B, (int)per, (int)N,
-                         (uint32_t)pages, (uint32_t)heads, (uint32_t)page};
+    const Batch batch = make_batch(table, starts, lens, B, per, N, pages, heads, page);
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((N + tokens - 1) / tokens)), dim3(kThreads), 0,
                            (hipStream_t)stream, Rows{(const uint16_t*)q, q_stride},
