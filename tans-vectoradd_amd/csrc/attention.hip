@@ -27,6 +27,9 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.44269504f;
 constexpr float kNone = -INFINITY;   // the maximum of nothing
 
+// The item that a workgroup's run ends in, if it begins there too and others go on with it.
+struct Cut { int start, rows, tile, h, last; };   // last: the workgroup that has its end, or -1
+
 struct Args {
     Batch batch;
     const uint16_t* q;
@@ -39,6 +42,7 @@ struct Args {
     uint16_t* out;
     Work work;
     float* parts;          // of split items: [workgroups][2][rows][D], then [workgroups][2][rows][2]
+    Cut* cuts;             // [workgroups]
 };
 
 // A sequence's part in the work: its row tiles and the slots' units.
@@ -70,26 +74,14 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
 }
 
-// The work of all sequences, and that of those before b.
-__device__ __forceinline__ void total_cost(const Args& a, int b, int64_t& all, int64_t& before) {
-    const int lane = threadIdx.x & (kLanes - 1);
-    all = before = 0;
-    if (a.batch.B == 1) {
-        all = uniform(cost(a, 0));
-        return;
-    }
-    for (int i = lane; i < a.batch.B; i += kLanes) {
-        const int64_t c = cost(a, i);
-        all += c;
-        before += i < b ? c : 0;
-    }
+// The work of all sequences.
+__device__ __forceinline__ int64_t total_cost(const Args& a) {
+    if (a.batch.B == 1) return uniform(cost(a, 0));
+    int64_t all = 0;
+    for (int i = threadIdx.x & (kLanes - 1); i < a.batch.B; i += kLanes) all += cost(a, i);
     #pragma unroll
-    for (int i = 1; i < kLanes; i *= 2) {
-        all += __shfl_xor(all, i);
-        before += __shfl_xor(before, i);
-    }
-    all = uniform(all);
-    before = uniform(before);
+    for (int i = 1; i < kLanes; i *= 2) all += __shfl_xor(all, i);
+    return uniform(all);
 }
 
 // The sequence that piece `at` < all of the work belongs to; at becomes the piece's
@@ -496,14 +488,15 @@ struct Item {
 };
 struct Run {
     int64_t left, in;   // pieces; the next one's number in its sequence
-    int b;
+    int64_t all, at;    // all of the work; the next piece
+    int b, groups;
     Seq s;
     __device__ __forceinline__ bool begin(const Args& a) {
-        int64_t all, none;
-        total_cost(a, 0, all, none);
-        const int groups = a.work.whole ? 0 : work_groups(a.work, all);
+        all = total_cost(a);
+        groups = a.work.whole ? 0 : work_groups(a.work, all);
+        if (!a.work.whole && threadIdx.x == 0) a.cuts[blockIdx.x].last = -1;
         if (a.work.whole ? (int64_t)blockIdx.x >= all : (int)blockIdx.x >= groups) return false;
-        in = a.work.whole ? (int64_t)blockIdx.x : range_start(all, groups, blockIdx.x);
+        in = at = a.work.whole ? (int64_t)blockIdx.x : range_start(all, groups, blockIdx.x);
         left = a.work.whole ? 1 : range_start(all, groups, blockIdx.x + 1) - in;
         b = find_piece(a, in);
         s = sequence(a, b);
@@ -531,8 +524,11 @@ struct Run {
         o.end = to - a.work.item;   // (none of its units if not above first)
         o.whole = o.first == 0 && o.end == s.units;
         o.cut = o.first > 0;
+        if (!o.cut && o.end > 0 && !o.whole && threadIdx.x == 0)
+            a.cuts[blockIdx.x] = {s.start, s.tokens * a.G, o.tile, o.h, range_of(all, groups, at - from + pieces - 1)};
         left -= to - from;
         in += to - from;
+        at += to - from;
         return o;
     }
     // The next item's sequence; false if there is none.
@@ -573,34 +569,46 @@ __device__ __forceinline__ Lookup look_up(const Args& a, const Run& run, int u, 
     return o;
 }
 
-// Loads a unit's rows (of nothing: row 0's, which no lane sees) into a stage, its share
-// if the workgroup's NW waves share it; returns the slots that exist.
+// Loads a unit's rows (of nothing: row 0's, which no lane sees) into a stage, or where NW
+// waves share it a wave's part of them.  find() says which rows a lane's loads take and
+// returns the slots that exist; it goes through LDS, so the loads come later.
 template <int D, bool FP8, int NW>
-__device__ __forceinline__ uint32_t load_unit(const Args& a, const Lookup& o, int h, Lds stage, Lds scales) {
+struct Loads {
     using T = Tile<D, FP8>;
-    constexpr int kLoads = 2 * T::loads / NW, kDistinct = NW > 1 ? kLoads : T::loads;
-    static_assert(2 * T::loads % NW == 0, "loads");
-    const int lane = threadIdx.x & (kLanes - 1);
-    const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes) : 0;
-    const bool valid = o.in && o.entry < a.batch.pages;
-    const uint32_t row = valid ? (o.entry * a.batch.heads + h) * a.batch.page + o.off : 0;
-    const uint32_t exists = (uint32_t)__builtin_amdgcn_ballot_w64(valid);
-    // K's loads, then V's; the rows that a lane loads come from their lanes
-    auto of = [&](int i) { return (wave * kLoads + i) % T::loads * T::per_load + lane / T::pieces; };
-    uint32_t from[kDistinct];
-    #pragma unroll
-    for (int i = 0; i < kDistinct; i++) from[i] = __shfl(row, of(i));
-    #pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-        const int n = wave * kLoads + i;
-        const bool is_v = n >= T::loads;
-        const uint32_t at = of(i % kDistinct), key = is_v ? T::key_of_v(at) : T::key_of_k(at);
-        load_lds<16>((is_v ? a.v : a.k) + (int64_t)from[i % kDistinct] * T::RB + ((lane % T::pieces) ^ key) * 16,
-                     stage + n * 1024);
+    // (units of fewer loads than waves: two waves load the same)
+    static constexpr int kLoads = 2 * T::loads > NW ? 2 * T::loads / NW : 1;
+    static constexpr int kDistinct = kLoads < T::loads ? kLoads : T::loads;
+    static constexpr int kIssue = kLoads + (FP8 ? 1 : 0);   // with the scales'
+    static_assert(kLoads == 1 || 2 * T::loads % NW == 0, "loads");
+    uint32_t from[kDistinct], mine;
+    // the i-th load's number in the stage, K's and then V's
+    static __device__ __forceinline__ int number(int i) {
+        const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes) : 0;
+        return (wave * kLoads + i) % (2 * T::loads);
     }
-    if constexpr (FP8) load_lds<4>((lane >> 5 ? a.v_scale : a.k_scale) + row, scales);
-    return exists;
-}
+    static __device__ __forceinline__ int row_of(int i) {
+        return number(i) % T::loads * T::per_load + (threadIdx.x & (kLanes - 1)) / T::pieces;
+    }
+    __device__ __forceinline__ uint32_t find(const Args& a, const Lookup& o, int h) {
+        const bool valid = o.in && o.entry < a.batch.pages;
+        mine = valid ? (o.entry * a.batch.heads + h) * a.batch.page + o.off : 0;
+        #pragma unroll
+        for (int i = 0; i < kDistinct; i++) from[i] = __shfl(mine, row_of(i));
+        return (uint32_t)__builtin_amdgcn_ballot_w64(valid);
+    }
+    __device__ __forceinline__ void issue(const Args& a, Lds stage, Lds scales) const {
+        const int lane = threadIdx.x & (kLanes - 1);
+        #pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int n = number(i);
+            const bool is_v = n >= T::loads;
+            const uint32_t at = row_of(i), key = is_v ? T::key_of_v(at) : T::key_of_k(at);
+            load_lds<16>((is_v ? a.v : a.k) + (int64_t)from[i % kDistinct] * T::RB + ((lane % T::pieces) ^ key) * 16,
+                         stage + n * 1024);
+        }
+        if constexpr (FP8) load_lds<4>((lane >> 5 ? a.v_scale : a.k_scale) + mine, scales);
+    }
+};
 
 // Where an item's sums go: to `out`, or to its part.
 struct Target {
@@ -626,7 +634,7 @@ template <int D, bool FP8, int RT, int NW, int STAGES>
 __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
     using T = Tile<D, FP8>;
     constexpr int kRows = 32 * RT;
-    constexpr int kIssue = 2 * T::loads + (FP8 ? 1 : 0);   // a unit's loads, with the scales'
+    constexpr int kIssue = Loads<D, FP8, 1>::kIssue;
     constexpr int kStage = 2 * T::bytes + (FP8 ? 256 : 0);
     constexpr int kRing = kStage * NW;
     __shared__ __attribute__((aligned(1024))) uint8_t ring0[kRing], ring1[kRing],
@@ -678,7 +686,9 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
             const Lookup l = la;
             la = lb;
             lb = look_up(a, run, v + 2 * NW, stop);
-            exists[i] = load_unit<D, FP8, 1>(a, l, o.h, rings[i] + mine, rings[i] + mine + 2 * T::bytes);
+            Loads<D, FP8, 1> loads;
+            exists[i] = loads.find(a, l, o.h);
+            loads.issue(a, rings[i] + mine, rings[i] + mine + 2 * T::bytes);
         };
         auto begin = [&](int v) {
             la = look_up(a, run, v, stop);
@@ -792,21 +802,17 @@ __global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
     } while (run.go_on(a));
 }
 
-// Many rows: each of four waves takes 32 RT rows of the tile and all units, which pass
-// through LDS once for all four.  The products of one part run beside the exponentials of
-// another, in one wave's own instructions, step by step (a step is a matrix instruction
-// and what fits beside it):
-//
-//   RT = 2   the row tiles take turns: the products of tile 0 (K's with the next unit, V's
-//            with this one) beside the exponentials of tile 1, then the other way around.
-//            Operands of K and V are read from LDS once for both.
-//   RT = 1   the next unit's products with K beside this one's exponentials, then V's.
-template <int D, bool FP8, int RT>
-__global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
+// Many rows: each of NW waves takes 32 rows of the tile and all units, which pass through
+// LDS once for all of them.  A unit's products with K run beside the exponentials of the
+// one before in the same wave's instructions, step by step (a step is a matrix instruction
+// and what goes beside it), and where the registers hold it (WAVES) two waves a SIMD fill
+// each other's gaps.
+template <int D, bool FP8, int NW, int WAVES>
+__global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a) {
     using T = Tile<D, FP8>;
-    constexpr int NW = 4, STAGES = 4;
-    constexpr int kRows = 32 * RT * NW;
-    constexpr int kIssue = 2 * T::loads / NW + (FP8 ? 1 : 0);   // a wave's loads of a unit
+    constexpr int STAGES = 4;
+    constexpr int kRows = 32 * NW;
+    constexpr int kIssue = Loads<D, FP8, NW>::kIssue;
     constexpr int kStage = 2 * T::bytes + (FP8 ? 256 * NW : 0);
     constexpr int kSteps = D / 16;   // products with K, and with V, of a unit and 32 rows
     __shared__ __attribute__((aligned(1024))) uint8_t ring0[kStage], ring1[kStage], ring2[kStage], ring3[kStage];
@@ -824,82 +830,79 @@ __global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
         const Item o = run.take(a);
         if (o.end <= o.first) continue;
         const Seq& s = run.s;
-        const int rows = s.tokens * a.G, row0 = o.tile * kRows + wave * 32 * RT;
+        const int rows = s.tokens * a.G, row = o.tile * kRows + wave * 32 + r;
         const int stop = run.stop(a, o, kRows), plain = run.plain(a, o, kRows, stop);
-        v8bf q[RT][D / 16];
-        Mask mask[RT];
-        Sums<D> sums[RT];
-        #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int row = row0 + 32 * t + r;
-            mask[t].token = row < rows ? row / a.G : -1;
-            mask[t].start = s.start;
-            load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask[t].token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
-                               row < rows, q[t]);
-            sums[t].clear();
-        }
+        v8bf q[D / 16];
+        Mask mask;
+        Sums<D> sums;
+        mask.token = row < rows ? row / a.G : -1;
+        mask.start = s.start;
+        load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask.token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
+                           row < rows, q);
+        sums.clear();
         uint32_t exists[STAGES];
         Lookup la, lb;
-        auto fetch = [&](int v, int i) {   // unit v, whose lookup is la, into stage i
+        Loads<D, FP8, NW> loads;
+        auto find = [&](int v, int i) {   // unit v, whose lookup is la, into stage i
             const Lookup l = la;
             la = lb;
             lb = look_up(a, run, v + 2, stop);
-            exists[i] = load_unit<D, FP8, NW>(a, l, o.h, rings[i], rings[i] + my_scales);
+            exists[i] = loads.find(a, l, o.h);
         };
+        auto issue = [&](int i) { loads.issue(a, rings[i], rings[i] + my_scales); };
         auto begin = [&](int v) {
             la = look_up(a, run, v, stop);
             lb = look_up(a, run, v + 1, stop);
             #pragma unroll
-            for (int i = 0; i < STAGES; i++) fetch(v + i, i);
+            for (int i = 0; i < STAGES; i++) {
+                find(v + i, i);
+                issue(i);
+            }
         };
         int u = o.first;
         if (u < stop) begin(u);
 
         // Plain units: the first, and then rounds of the stages.
         uint32_t whole = 0xFFFFFFFFu;
-        const int rounds = plain > u ? (plain - u - 1) / STAGES : 0;
         if (plain > u) {
             v16f sc[2];
-            v4u kr[kSteps], vr[kSteps];       // operands as they were read
-            v8bf kf[kSteps], vf[kSteps];      // and as the products take them
+            v4u kr[kSteps], vr[kSteps];   // operands (8 bits: as they were read)
             float ks[FP8 ? 16 : 1], vs[FP8 ? 16 : 1], e[16], mc = 0.0f;
-            uint32_t p[RT][8];
+            uint32_t p[8];
             auto read_k = [&](Lds stage, int j) {
                 if (!FP8 || j % 2 == 0) kr[j] = at.read_k(stage, j);
             };
             auto read_v = [&](Lds stage, int x) { vr[x] = at.read_v(stage, x % (D / 32), x / (D / 32)); };
-            auto take_k = [&](int j) {
+            auto with_k = [&](v16f& to, int j) {
                 const v4u& x = kr[FP8 ? j / 2 * 2 : j];
-                kf[j] = FP8 ? from_fp8(x[2 * (j % 2)], x[2 * (j % 2) + 1]) : __builtin_bit_cast(v8bf, x);
-            };
-            auto take_v = [&](int x) { vf[x] = FP8 ? from_fp8(vr[x][0], vr[x][1]) : __builtin_bit_cast(v8bf, vr[x]); };
-            auto with_k = [&](v16f& to, int t, int j) {
                 v16f zero = {};
-                to = mfma(kf[j], q[t][j], j == 0 ? zero : to);
+                to = mfma(FP8 ? from_fp8(x[2 * (j % 2)], x[2 * (j % 2) + 1]) : __builtin_bit_cast(v8bf, x), q[j],
+                          j == 0 ? zero : to);
             };
-            auto with_v = [&](int t, int x) {
-                const uint32_t* w = p[t] + x / (D / 32) * 4;
-                sums[t].acc[x % (D / 32)] = mfma(vf[x], __builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]}),
-                                                 sums[t].acc[x % (D / 32)]);
+            auto with_v = [&](int x) {
+                const uint32_t* w = p + x / (D / 32) * 4;
+                v16f& to = sums.acc[x % (D / 32)];
+                to = mfma(FP8 ? from_fp8(vr[x][0], vr[x][1]) : __builtin_bit_cast(v8bf, vr[x]),
+                          __builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]}), to);
             };
             auto step = [] {
                 __builtin_amdgcn_sched_barrier(0);
                 asm volatile("" ::: "memory");
             };
-            // Softmax of tile t's scores, in steps 0 .. n - 1.
-            auto softmax = [&](v16f& x, int t, int i, int n) {
+            // the exponentials of a unit's scores, in steps 0 .. kSteps - 1
+            auto softmax = [&](v16f& x, int i) {
                 if (i == 0) {
                     if constexpr (FP8)
                         #pragma unroll
                         for (int c = 0; c < 16; c++) x[c] *= ks[c];
-                    mc = sums[t].admit(x, a.c);
+                    mc = sums.admit(x, a.c);
                 } else {
                     #pragma unroll
-                    for (int c = 16 * (i - 1) / (n - 1); c < 16 * i / (n - 1); c++) {
+                    for (int c = 16 * (i - 1) / (kSteps - 1); c < 16 * i / (kSteps - 1); c++) {
                         e[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c], a.c, -mc));
-                        sums[t].l += e[c];
+                        sums.l += e[c];
                         if constexpr (FP8) e[c] *= vs[c];
-                        if (c % 2) p[t][c / 2] = bf16_pack(e[c - 1], e[c]);
+                        if (c % 2) p[c / 2] = bf16_pack(e[c - 1], e[c]);
                     }
                 }
             };
@@ -915,101 +918,50 @@ __global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
             for (int j = 0; j < kSteps; j++) read_k(rings[0], j);
             scales(rings[0]);
             #pragma unroll
-            for (int j = 0; j < kSteps; j++) {
-                take_k(j);
-                with_k(sc[0], 0, j);
-                if constexpr (RT == 2) with_k(sc[1], 1, j);
-            }
+            for (int j = 0; j < kSteps; j++) with_k(sc[0], j);
             whole &= exists[0];
             #pragma unroll
-            for (int j = 0; j < kSteps; j++) {
-                read_k(rings[1], j);
-                if constexpr (RT == 2) read_v(rings[0], j);
-            }
-            if constexpr (RT == 2) {
+            for (int j = 0; j < kSteps; j++) read_k(rings[1], j);
+            for (int n = (plain - u - 1) / STAGES; n > 0; n--) {
                 #pragma unroll
-                for (int i = 0; i < 2 * kSteps; i++) softmax(sc[0], 0, i, 2 * kSteps);
-            }
-            for (int n = 0; n < rounds; n++) {
-                #pragma unroll
-                for (int i = 0; i < STAGES; i++) {   // unit u, in stage i
-                    const Lds st1 = rings[(i + 1) % STAGES], st2 = rings[(i + 2) % STAGES];
-                    if constexpr (RT == 2) {
-                        #pragma unroll
-                        for (int j = 0; j < 2 * kSteps; j++) {
-                            if (j < kSteps) {
-                                take_k(j);
-                                with_k(sc[0], 0, j);
-                            } else {
-                                take_v(j - kSteps);
-                                with_v(0, j - kSteps);
-                            }
-                            softmax(sc[1], 1, j, 2 * kSteps);
-                            step();
+                for (int i = 0; i < STAGES; i++, u++) {   // unit u, in stage i
+                    whole &= exists[(i + 1) % STAGES];
+                    #pragma unroll
+                    for (int j = 0; j < kSteps; j++) {
+                        with_k(sc[(i + 1) % 2], j);
+                        softmax(sc[i % 2], j);
+                        // (LDS answers in order: find() after K's reads, before V's)
+                        constexpr int kAt = kSteps / 4;
+                        if (j == kAt) find(u + STAGES, i);
+                        if (j > kAt && 2 * (j - kAt - 1) < kSteps) {
+                            read_v(rings[i], 2 * (j - kAt - 1));
+                            read_v(rings[i], 2 * (j - kAt - 1) + 1);
                         }
-                        whole &= exists[(i + 1) % STAGES];
-                        arrive<kIssue>();   // unit u + 2; unit u has been read
-                        scales(st1);
-                        fetch(u + STAGES, i);
-                        #pragma unroll
-                        for (int j = 0; j < 2 * kSteps; j++) {
-                            if (j < kSteps) {
-                                with_k(sc[1], 1, j);
-                                softmax(sc[0], 0, j, 2 * kSteps);
-                                read_k(st2, j);
-                            } else {
-                                with_v(1, j - kSteps);
-                                softmax(sc[0], 0, j, 2 * kSteps);
-                                read_v(st1, j - kSteps);
-                            }
-                            step();
-                        }
-                    } else {
-                        #pragma unroll
-                        for (int j = 0; j < kSteps; j++) {
-                            take_k(j);
-                            with_k(sc[(i + 1) % 2], 0, j);
-                            softmax(sc[i % 2], 0, j, kSteps);
-                            if (2 * j < kSteps) {
-                                read_v(rings[i], 2 * j);
-                                read_v(rings[i], 2 * j + 1);
-                            }
-                            step();
-                        }
-                        whole &= exists[(i + 1) % STAGES];
-                        arrive<kIssue>();   // unit u + 2; unit u has been read
-                        fetch(u + STAGES, i);
-                        #pragma unroll
-                        for (int j = 0; j < kSteps; j++) {
-                            take_v(j);
-                            with_v(0, j);
-                            read_k(st2, j);
-                            if (j == 0) scales(st1);
-                            step();
-                        }
+                        step();
                     }
-                    u++;
+                    arrive<kIssue>();   // unit u + 2; unit u has been read
+                    issue(i);
+                    #pragma unroll
+                    for (int j = 0; j < kSteps; j++) {
+                        with_v(j);
+                        read_k(rings[(i + 2) % STAGES], j);
+                        if (j == 0) scales(rings[(i + 1) % STAGES]);
+                        step();
+                    }
                 }
             }
             // the last one's rest
-            if constexpr (RT == 1) {
-                #pragma unroll
-                for (int x = 0; x < kSteps; x++) read_v(rings[0], x);
-            }
             #pragma unroll
-            for (int i = 0; i < 2 * kSteps; i++) softmax(sc[RT - 1], RT - 1, i, 2 * kSteps);
+            for (int x = 0; x < kSteps; x++) read_v(rings[0], x);
             #pragma unroll
-            for (int x = 0; x < kSteps; x++) {
-                take_v(x);
-                #pragma unroll
-                for (int t = 0; t < RT; t++) with_v(t, x);
-            }
+            for (int i = 0; i < kSteps; i++) softmax(sc[0], i);
+            #pragma unroll
+            for (int x = 0; x < kSteps; x++) with_v(x);
             u++;
             arrive<0>();   // (before the ring is filled again)
             if (__builtin_amdgcn_readfirstlane(whole) != 0xFFFFFFFFu) {
                 // some of them were of pages that do not exist: all over again, slot by slot
-                #pragma unroll
-                for (int t = 0; t < RT; t++) sums[t].clear();
+                sums.clear();
                 u = o.first;
             }
             if (u < stop) begin(u);
@@ -1019,34 +971,29 @@ __global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
             arrive<0>();
             for (int i = 0; i < STAGES && u < stop; i++, u++) {
                 const Lds stage = i == 0 ? rings[0] : i == 1 ? rings[1] : i == 2 ? rings[2] : rings[3];
-                uint32_t e = exists[0];
+                mask.before = s.context - u * kUnit;
+                mask.exists = exists[0];
                 #pragma unroll
-                for (int k = 1; k < STAGES; k++) e = i == k ? exists[k] : e;
-                #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    mask[t].before = s.context - u * kUnit;
-                    mask[t].exists = e;
-                    attend_unit<D, FP8, true>(a, at, stage, stage + my_scales, q[t], sums[t], mask[t]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    asm volatile("" ::: "memory");
-                }
+                for (int k = 1; k < STAGES; k++) mask.exists = i == k ? exists[k] : mask.exists;
+                attend_unit<D, FP8, true>(a, at, stage, stage + my_scales, q, sums, mask);
             }
             arrive<0>();   // (before the ring is filled again)
             if (u < stop) {
                 #pragma unroll
-                for (int i = 0; i < STAGES; i++) fetch(u + i, i);
+                for (int i = 0; i < STAGES; i++) {
+                    find(u + i, i);
+                    issue(i);
+                }
             }
         }
 
         const Target to = target<D>(a, run, o, kRows);
-        #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const float l = sum_of(sums[t].l);
-            const int row = row0 + 32 * t + r, local = row - o.tile * kRows;
-            if (row >= rows) continue;
+        const float l = sum_of(sums.l);
+        const int local = row - o.tile * kRows;
+        if (row < rows) {
             const float by = l == 0.0f ? 0.0f : 1.0f / l;
             if (to.parts && g == 0) {
-                to.part_s[local * 2] = sums[t].m;
+                to.part_s[local * 2] = sums.m;
                 to.part_s[local * 2 + 1] = l;
             }
             uint16_t* out = to.out + out_row(a, run, o, row) * D;
@@ -1055,7 +1002,7 @@ __global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
                 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int d = 32 * n + 8 * i + 4 * g;
-                    const v16f& c = sums[t].acc[n];
+                    const v16f& c = sums.acc[n];
                     const v4f x = {c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]};
                     if (to.parts)
                         *reinterpret_cast<v4f*>(to.part_o + local * D + d) = x;
@@ -1066,43 +1013,60 @@ __global__ __launch_bounds__(4 * kLanes, 1) void attend_rows_kernel(Args a) {
     } while (run.go_on(a));
 }
 
-// The rows of items that several workgroups share, from their parts in the order of
-// the slots.  A wave takes a row.
+// The rows of items that several workgroups share, from their parts in the order of the
+// slots: kJoins workgroups (y) for each run that could be the first of several (x), which
+// take the rows in runs.  A thread has 4 dimensions of a part, of as many parts at a time
+// as there are threads for, and where the parts are few, of several rows.
+constexpr int kJoins = 32;
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
-    const int lane = threadIdx.x & (kLanes - 1);
-    const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-    const int n = (int)(id / a.Hq), hq = (int)(id % a.Hq);
-    if (n >= a.batch.N) return;
-    const int b = find_sequence(a.batch, n);
-    if (b < 0 || n >= a.batch.start(b + 1)) return;
-    const Seq s = sequence(a, b);
-    int64_t all, before;
-    total_cost(a, b, all, before);
-    const int groups = work_groups(a.work, all);
-    const int h = hq / a.G, row = (n - s.start) * a.G + hq % a.G;
-    const int tile = row / a.work.rows, local = row % a.work.rows;
-    const int64_t from = before + ((int64_t)h * s.tiles + tile) * (s.units + a.work.item) + a.work.item,
-                  to = from + s.units;
-    const int w0 = range_of(all, groups, from), w1 = range_of(all, groups, to - 1);
-    if (w0 == w1) return;   // (one workgroup had the whole item)
-    constexpr int E = D / kLanes;
+    const Cut cut = a.cuts[blockIdx.x];
+    const int rows = a.work.rows / kJoins, first = (int)blockIdx.y * rows;
+    const int end = min(min(a.work.rows, cut.rows - cut.tile * a.work.rows), first + rows);
+    if (cut.last < 0 || first >= end) return;
+    constexpr int T = D / 4, kTeams = 256 / T;   // threads of a row's part
+    __shared__ __attribute__((aligned(16))) float sums[kTeams][D], total[kTeams];
+    const int w0 = blockIdx.x, n = cut.last - w0 + 1;
+    // teams that share a row: as many as there are parts, a power of two
+    int share = 1;
+    while (share < n && share < kTeams) share *= 2;
     const float* stats = a.parts + (int64_t)a.work.groups * 2 * a.work.rows * D;
-    auto slot = [&](int w) { return ((int64_t)w * 2 + (from < range_start(all, groups, w) ? 0 : 1)) * a.work.rows + local; };
-    float top = kNone;
-    for (int w = w0; w <= w1; w++) top = fmaxf(top, stats[slot(w) * 2]);
-    float sum = 0.0f, o[E] = {};
-    for (int w = w0; w <= w1; w++) {
-        const float m = stats[slot(w) * 2];
-        const float by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.c);
-        sum += stats[slot(w) * 2 + 1] * by;
-        #pragma unroll
-        for (int i = 0; i < E; i++) o[i] += a.parts[slot(w) * D + lane * E + i] * by;
+    const int team = threadIdx.x / T, t = threadIdx.x % T, mine = team % share;
+    for (int row0 = first; row0 < end; row0 += kTeams / share) {
+        const int local = row0 + team / share;
+        if (local < end) {
+            // (a run's first item is its part 0 if it began in another's, its last one part 1)
+            auto slot = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * a.work.rows + local; };
+            float top = kNone;
+            #pragma unroll 4
+            for (int i = 0; i < n; i++) top = fmaxf(top, stats[slot(i) * 2]);
+            float sum = 0.0f;
+            v4f o = {0, 0, 0, 0};
+            #pragma unroll 4
+            for (int i = mine; i < n; i += share) {
+                const float m = stats[slot(i) * 2];
+                const float by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.c);
+                sum += stats[slot(i) * 2 + 1] * by;
+                o += *reinterpret_cast<const v4f*>(a.parts + slot(i) * D + t * 4) * by;
+            }
+            *reinterpret_cast<v4f*>(&sums[team][t * 4]) = o;
+            if (t == 0) total[team] = sum;
+        }
+        __syncthreads();
+        if (local < end && mine == 0) {
+            float sum = 0.0f;
+            v4f o = {0, 0, 0, 0};
+            for (int i = 0; i < share; i++) {
+                sum += total[team + i];
+                o += *reinterpret_cast<const v4f*>(&sums[team + i][t * 4]);
+            }
+            const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int row = cut.tile * a.work.rows + local;
+            uint16_t* out = a.out + ((int64_t)(cut.start + row / a.G) * a.Hq + cut.h * a.G + row % a.G) * D + t * 4;
+            *reinterpret_cast<v2u*>(out) = v2u{bf16_pack(o[0] * by, o[1] * by), bf16_pack(o[2] * by, o[3] * by)};
+        }
+        __syncthreads();
     }
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t* out = a.out + ((int64_t)n * a.Hq + hq) * D + lane * E;
-    #pragma unroll
-    for (int i = 0; i < E; i++) out[i] = (uint16_t)bf16_pack(o[i] * by, 0.0f);
 }
 
 }  // namespace
@@ -1162,6 +1126,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
     a.out = (uint16_t*)out;
     a.work = p.work;
     a.parts = (float*)workspace;
+    a.cuts = (Cut*)((char*)workspace + p.parts_bytes);
     auto launch = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)p.blocks), dim3(threads), 0, (hipStream_t)stream, a);
         return hip_check(hipGetLastError(), "attend_kernel launch");
@@ -1174,18 +1139,17 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         constexpr int stages = 4 * stage <= (132 << 10) ? 4 : 2;
         int rc;
         if (p.kind == kFew) rc = launch(attend_kernel<D, f8, 1, nw, stages>, nw * kLanes);
-        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 1>, 4 * kLanes);
+        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 4, 1>, 4 * kLanes);
         else {
             if constexpr (D < 256) {
                 if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages>, nw * kLanes);
-                else rc = launch(attend_rows_kernel<D, f8, 2>, 4 * kLanes);
+                else rc = launch(attend_rows_kernel<D, f8, 8, 2>, 8 * kLanes);
             } else {
                 rc = fail(TANS_EINVAL, "tree_attention: no such kernel");   // (not reached: plan())
             }
         }
-        if (rc == TANS_OK && !p.work.whole) {
-            hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)((N * q_heads + 3) / 4)), dim3(256), 0,
-                               (hipStream_t)stream, a);
+        if (rc == TANS_OK && !p.work.whole && p.work.groups > 1) {
+            hipLaunchKernelGGL(join_kernel<D>, dim3(p.work.groups - 1, kJoins), dim3(256), 0, (hipStream_t)stream, a);
             rc = hip_check(hipGetLastError(), "join_kernel launch");
         }
         return rc;

@@ -58,7 +58,7 @@ enum Kind { kFew, kSome, kMany, kMost };
 struct Plan {
     Kind kind;
     Work work;
-    int64_t blocks, bytes;   // workgroups; of the parts
+    int64_t blocks, parts_bytes, bytes;   // workgroups; of the parts; of the workspace
 };
 
 inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, int64_t slots,
@@ -77,8 +77,9 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
         return p;
     }
     p.work.groups = cus;
-    p.blocks = cus;
-    p.bytes = (int64_t)p.work.groups * 2 * p.work.rows * (dim + 2) * 4;
+    p.blocks = p.work.groups;
+    p.parts_bytes = (int64_t)p.work.groups * 2 * p.work.rows * (dim + 2) * 4;
+    p.bytes = p.parts_bytes + (int64_t)p.work.groups * 5 * 4;
     return p;
 }
 
