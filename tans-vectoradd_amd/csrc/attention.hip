@@ -630,8 +630,8 @@ __device__ __forceinline__ int64_t out_row(const Args& a, const Run& run, const 
 // ring of its own in LDS that loads write without a register between; the waves' sums are
 // added at the end.  Nothing makes the waves wait for each other, so that each keeps its
 // ring's loads under way.
-template <int D, bool FP8, int RT, int NW, int STAGES>
-__global__ __launch_bounds__(NW * kLanes, 1) void attend_kernel(Args a) {
+template <int D, bool FP8, int RT, int NW, int STAGES, int WAVES>
+__global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
     using T = Tile<D, FP8>;
     constexpr int kRows = 32 * RT;
     constexpr int kIssue = Loads<D, FP8, 1>::kIssue;
@@ -1081,7 +1081,8 @@ int tans_tree_attention_workspace(int64_t N, int64_t B, int64_t q_heads, int64_t
         N > INT32_MAX / 2 || B >= INT32_MAX)
         return fail(TANS_EINVAL, "tree_attention: sizes out of range");
     const int cus = tans_internal_cu_count();
-    *bytes = N && B ? plan(N, B, q_heads, heads, dim, slots, max_tokens, cus > 0 ? cus : 256).bytes : 0;
+    // (an 8-bit cache takes no less)
+    *bytes = N && B ? plan(N, B, q_heads, heads, dim, true, slots, max_tokens, cus > 0 ? cus : 256).bytes : 0;
     return TANS_OK;
 }
 
@@ -1106,7 +1107,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
     if (rc != TANS_OK) return rc;
     const int cus = tans_internal_cu_count();
     if (cus <= 0) return fail(TANS_EHIP, op + ": cannot query the device's CU count");
-    const Plan p = plan(N, B, q_heads, heads, dim, per * page, max_tokens, cus);
+    const Plan p = plan(N, B, q_heads, heads, dim, k_scale != nullptr, per * page, max_tokens, cus);
     if (p.bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes))
         return fail(TANS_EINVAL, op + ": workspace too small, null or misaligned (16 bytes)");
     if (p.blocks > INT32_MAX / 256) return fail(TANS_EINVAL, op + ": too many tokens for one call");
@@ -1137,12 +1138,18 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         constexpr int nw = D == 256 && !f8 ? 2 : 4;
         constexpr int stage = (2 * Tile<D, f8>::bytes + (f8 ? 256 : 0)) * nw;
         constexpr int stages = 4 * stage <= (132 << 10) ? 4 : 2;
+        constexpr int pair_stages = 2 * stages * stage <= (160 << 10) ? stages : 2;
         int rc;
-        if (p.kind == kFew) rc = launch(attend_kernel<D, f8, 1, nw, stages>, nw * kLanes);
+        if (p.kind == kFew) {
+            rc = TANS_EINVAL;
+            if constexpr (few_pairs(D, f8))
+                if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2>, nw * kLanes);
+            if (!p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, stages, 1>, nw * kLanes);
+        }
         else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 4, 1>, 4 * kLanes);
         else {
             if constexpr (D < 256) {
-                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages>, nw * kLanes);
+                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1>, nw * kLanes);
                 else rc = launch(attend_rows_kernel<D, f8, 8, 2>, 8 * kLanes);
             } else {
                 rc = fail(TANS_EINVAL, "tree_attention: no such kernel");   // (not reached: plan())

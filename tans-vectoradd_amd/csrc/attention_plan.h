@@ -58,11 +58,15 @@ enum Kind { kFew, kSome, kMany, kMost };
 struct Plan {
     Kind kind;
     Work work;
+    bool pairs;              // two workgroups a CU
     int64_t blocks, parts_bytes, bytes;   // workgroups; of the parts; of the workspace
 };
 
-inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, int64_t slots,
-                 int64_t max_tokens, int cus) {
+// Whether a CU's LDS holds the rings of two workgroups of the kernel for few rows.
+constexpr bool few_pairs(int64_t dim, bool eight) { return dim * (eight ? 1 : 2) <= 128; }
+
+inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, bool eight,
+                 int64_t slots, int64_t max_tokens, int cus) {
     const int64_t G = q_heads / heads, rows = max_tokens * G;
     Plan p = {};
     p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome : rows <= 128 || dim == 256 ? kMany : kMost;
@@ -70,13 +74,17 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
     // no more items than this
     const int64_t items = (N * G / p.work.rows + std::min(N, B)) * heads;
     p.work.least = 8;
-    p.work.item = 8;
+    p.work.item = p.kind >= kMany ? 8 : (int)(196608 / (2 * kUnit * dim * (eight ? 1 : 2)));
     p.work.whole = slots <= 8 * kUnit || (p.kind >= kMany && items >= 4 * (int64_t)cus);
     if (p.work.whole) {
         p.blocks = items;
         return p;
     }
-    p.work.groups = cus;
+    // Two workgroups a CU, of which one streams while the other begins or ends an item, but
+    // for items that are longer than a run.  D = 128 in 8 bits, two against one: 256 sequences
+    // of 512 slots 84 / 119 us, 96 of 100 .. 16000 140 / 137, one of 262144 120 / 110.
+    p.pairs = p.kind == kFew && few_pairs(dim, eight) && items > cus;
+    p.work.groups = p.pairs ? 2 * cus : cus;
     p.blocks = p.work.groups;
     p.parts_bytes = (int64_t)p.work.groups * 2 * p.work.rows * (dim + 2) * 4;
     p.bytes = p.parts_bytes + (int64_t)p.work.groups * 5 * 4;
