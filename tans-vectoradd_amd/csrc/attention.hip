@@ -351,7 +351,7 @@ __device__ __forceinline__ void read_scales(Lds from, float (&f)[16]) {
 struct Mask {
     int token;         // the lane's row's, in its sequence, or -1
     int start;         // the sequence's first row of q
-    int before;        // slots of the context from the unit's first on
+    int before;        // slots of the context from the unit's first on, 32 at most
     uint32_t exists;   // of the unit's slots
 };
 template <int D, bool FP8, bool MASKED>
@@ -669,7 +669,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
         auto compute = [&](auto MASKED, int u, uint32_t exists, Lds stage) {
             #pragma unroll
             for (int t = 0; t < RT; t++) {
-                mask[t].before = s.context - u * kUnit;
+                mask[t].before = min(s.context - u * kUnit, kUnit);
                 mask[t].exists = exists;
                 attend_unit<D, FP8, decltype(MASKED)::value>(a, at, stage + mine, stage + mine + 2 * T::bytes, q[t], sums[t], mask[t]);
                 // (the second tile reads the stage again: its operands in registers from one
@@ -971,7 +971,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
             arrive<0>();
             for (int i = 0; i < STAGES && u < stop; i++, u++) {
                 const Lds stage = i == 0 ? rings[0] : i == 1 ? rings[1] : i == 2 ? rings[2] : rings[3];
-                mask.before = s.context - u * kUnit;
+                mask.before = min(s.context - u * kUnit, kUnit);
                 mask.exists = exists[0];
                 #pragma unroll
                 for (int k = 1; k < STAGES; k++) mask.exists = i == k ? exists[k] : mask.exists;
@@ -1078,7 +1078,7 @@ int tans_tree_attention_workspace(int64_t N, int64_t B, int64_t q_heads, int64_t
     if (!bytes) return fail(TANS_EINVAL, "tree_attention: null pointer");
     if (N < 0 || B < 0 || heads < 1 || q_heads < heads || q_heads % heads || q_heads > 65535 ||
         (dim != 64 && dim != 128 && dim != 256) || slots < 0 || slots > INT32_MAX || max_tokens < 0 ||
-        N > INT32_MAX / 2 || B >= INT32_MAX)
+        N > INT32_MAX / 2 || N > INT32_MAX / q_heads || B >= INT32_MAX)
         return fail(TANS_EINVAL, "tree_attention: sizes out of range");
     const int cus = tans_internal_cu_count();
     // (an 8-bit cache takes no less)
@@ -1100,6 +1100,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         return fail(TANS_EINVAL, op + ": the mask must have 0 .. 2^31 - 1 columns");
     if (!(scale > 0.0f) || scale > 1.0e38f) return fail(TANS_EINVAL, op + ": scale must be positive and finite");
     if (max_tokens < 0) return fail(TANS_EINVAL, op + ": max_tokens must not be negative");
+    if (N > INT32_MAX / q_heads) return fail(TANS_EINVAL, op + ": N times the query heads must be below 2^31");
     if (N == 0 || B == 0) return TANS_OK;
     if (!q || !out) return fail(TANS_EINVAL, op + ": null pointer");
     rc = stride_check(op, "q", q, q_stride, q_heads * dim);
