@@ -1014,22 +1014,18 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
 }
 
 // The rows of items that several workgroups share, from their parts in the order of the
-// slots: kJoins workgroups (y) for each run that could be the first of several (x), which
-// take the rows in runs.  A thread has 4 dimensions of a part, of as many parts at a time
-// as there are threads for, and where the parts are few, of several rows.
-constexpr int kJoins = 32;
-template <int D>
+// slots: a workgroup for ROWS rows (y) of each run that could be the first of several (x).
+// A thread has 4 dimensions of a row's parts; threads that the rows leave share the parts.
+template <int D, int ROWS>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
     const Cut cut = a.cuts[blockIdx.x];
-    const int rows = a.work.rows / kJoins, first = (int)blockIdx.y * rows;
-    const int end = min(min(a.work.rows, cut.rows - cut.tile * a.work.rows), first + rows);
+    const int first = (int)blockIdx.y * ROWS;
+    const int end = min(min(a.work.rows, cut.rows - cut.tile * a.work.rows), first + ROWS);
     if (cut.last < 0 || first >= end) return;
     constexpr int T = D / 4, kTeams = 256 / T;   // threads of a row's part
     __shared__ __attribute__((aligned(16))) float sums[kTeams][D], total[kTeams];
     const int w0 = blockIdx.x, n = cut.last - w0 + 1;
-    // teams that share a row: as many as there are parts, a power of two
-    int share = 1;
-    while (share < n && share < kTeams) share *= 2;
+    constexpr int share = kTeams > ROWS ? kTeams / ROWS : 1;   // teams that share a row
     const float* stats = a.parts + (int64_t)a.work.groups * 2 * a.work.rows * D;
     const int team = threadIdx.x / T, t = threadIdx.x % T, mine = team % share;
     for (int row0 = first; row0 < end; row0 += kTeams / share) {
@@ -1038,11 +1034,11 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
             // (a run's first item is its part 0 if it began in another's, its last one part 1)
             auto slot = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * a.work.rows + local; };
             float top = kNone;
-            #pragma unroll 4
+            #pragma unroll 8
             for (int i = 0; i < n; i++) top = fmaxf(top, stats[slot(i) * 2]);
             float sum = 0.0f;
             v4f o = {0, 0, 0, 0};
-            #pragma unroll 4
+            #pragma unroll 8
             for (int i = mine; i < n; i += share) {
                 const float m = stats[slot(i) * 2];
                 const float by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.c);
@@ -1147,7 +1143,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
                 if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2>, nw * kLanes);
             if (!p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, stages, 1>, nw * kLanes);
         }
-        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 4, 1>, 4 * kLanes);
+        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 4, D < 256 ? 2 : 1>, 4 * kLanes);
         else {
             if constexpr (D < 256) {
                 if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1>, nw * kLanes);
@@ -1157,7 +1153,11 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
             }
         }
         if (rc == TANS_OK && !p.work.whole && p.work.groups > 1) {
-            hipLaunchKernelGGL(join_kernel<D>, dim3(p.work.groups - 1, kJoins), dim3(256), 0, (hipStream_t)stream, a);
+            auto join = [&](auto kernel, int rows) {
+                hipLaunchKernelGGL(kernel, dim3(p.work.groups - 1, p.work.rows / rows), dim3(256), 0, (hipStream_t)stream, a);
+            };
+            if (p.work.rows <= 64) join(join_kernel<D, 4>, 4);
+            else join(join_kernel<D, 8>, 8);
             rc = hip_check(hipGetLastError(), "join_kernel launch");
         }
         return rc;

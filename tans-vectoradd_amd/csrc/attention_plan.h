@@ -69,7 +69,7 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
                  int64_t slots, int64_t max_tokens, int cus) {
     const int64_t G = q_heads / heads, rows = max_tokens * G;
     Plan p = {};
-    p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome : rows <= 128 || dim == 256 ? kMany : kMost;
+    p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome : rows <= 128 || dim == 256 || ((rows + 127) / 128 % 2 == 1 && rows < 1024) ? kMany : kMost;
     p.work.rows = 32 << p.kind;
     // no more items than this
     const int64_t items = (N * G / p.work.rows + std::min(N, B)) * heads;
@@ -84,7 +84,7 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
     // for items that are longer than a run.  D = 128 in 8 bits, two against one: 256 sequences
     // of 512 slots 84 / 119 us, 96 of 100 .. 16000 140 / 137, one of 262144 120 / 110.
     p.pairs = p.kind == kFew && few_pairs(dim, eight) && items > cus;
-    p.work.groups = p.pairs ? 2 * cus : cus;
+    p.work.groups = p.pairs || (p.kind == kMany && dim < 256) ? 2 * cus : cus;
     p.blocks = p.work.groups;
     p.parts_bytes = (int64_t)p.work.groups * 2 * p.work.rows * (dim + 2) * 4;
     p.bytes = p.parts_bytes + (int64_t)p.work.groups * 5 * 4;
