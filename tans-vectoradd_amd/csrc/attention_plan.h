@@ -51,6 +51,11 @@ TANS_BOTH int range_of(int64_t all, int groups, int64_t at) {
     return (int)(((at + 1) * groups - 1) / all);
 }
 
+// The run of workgroup i of `groups`: workgroups go to the 8 XCDs in turn, and XCD x takes
+// the x-th eighth of the runs (all of them one by one where they do not divide).
+constexpr int kXcds = 8;
+TANS_BOTH int run_of(int i, int groups) { return groups % kXcds ? i : i % kXcds * (groups / kXcds) + i / kXcds; }
+
 // Rows of q of a tile: 32 or 64, of which each wave takes all and the waves share the
 // slots, or 128 or 256, of which each wave takes a quarter and the slots pass through
 // LDS once for all.
