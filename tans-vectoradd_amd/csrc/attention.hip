@@ -613,6 +613,60 @@ struct Loads {
     }
 };
 
+// The same where pages are multiples of 16 rows, so that each half of a unit, and with it
+// each load, lies in one page: pages are looked up and addresses computed once a wave, by
+// scalar instructions, and lanes add a constant.  For D = 256, whose waves have 8 loads a
+// unit (2048 tokens of a prompt 645 us through lanes' lookups, 593 so); with D = 128 and 2 loads
+// the scalar chain behind the barrier costs more than it saves (683 / 709), D = 64 442 / 512.
+template <int D, bool FP8, int NW>
+struct PagedLoads {
+    using T = Tile<D, FP8>;
+    using L = Loads<D, FP8, NW>;
+    uint32_t offset[L::kLoads];   // a lane's, from the first row of a load
+    uint32_t entry[2], off[2];    // the next unit's halves
+    bool in[2];
+    __device__ __forceinline__ void set() {
+        const int lane = threadIdx.x & (kLanes - 1);
+        #pragma unroll
+        for (int i = 0; i < L::kLoads; i++) {
+            const uint32_t at = L::row_of(i), key = L::number(i) >= T::loads ? T::key_of_v(at) : T::key_of_k(at);
+            offset[i] = lane / T::pieces * T::RB + ((lane % T::pieces) ^ key) * 16;
+        }
+    }
+    // (the table through the scalar cache: nothing writes to it meanwhile)
+    __device__ __forceinline__ void look_up(const Args& a, const Run& run, int u, int stop) {
+        const auto* table = (const __attribute__((address_space(4))) int32_t*)a.batch.table + (int64_t)run.b * a.batch.per;
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t slot = (uint32_t)u * kUnit + 16 * k;
+            in[k] = u < stop && slot < (uint32_t)run.s.slots;
+            const uint32_t i = in[k] ? a.batch.page_of(slot) : 0;
+            off[k] = in[k] ? slot - i * a.batch.page : 0;
+            entry[k] = (uint32_t)table[i];
+        }
+    }
+    // Loads the unit that was looked up; whether all of its slots exist.
+    __device__ __forceinline__ bool issue(const Args& a, int h, Lds stage, Lds scales) const {
+        const int lane = threadIdx.x & (kLanes - 1);
+        uint32_t row[2];
+        bool all = true;
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const bool valid = in[k] && entry[k] < a.batch.pages;
+            row[k] = valid ? (entry[k] * a.batch.heads + h) * a.batch.page + off[k] : 0;
+            all = all && valid;
+        }
+        #pragma unroll
+        for (int i = 0; i < L::kLoads; i++) {
+            const int n = L::number(i), first = n % T::loads * T::per_load;
+            const uint32_t from = (first >= 16 ? row[1] : row[0]) + first % 16;
+            load_lds<16>((n >= T::loads ? a.v : a.k) + (int64_t)from * T::RB + offset[i], stage + n * 1024);
+        }
+        if constexpr (FP8) load_lds<4>((lane >> 5 ? a.v_scale : a.k_scale) + (lane & 16 ? row[1] : row[0]) + (lane & 15), scales);
+        return all;
+    }
+};
+
 // Where an item's sums go: to `out`, or to its part.
 struct Target {
     uint16_t* out;
@@ -810,7 +864,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
 // one before in the same wave's instructions, step by step (a step is a matrix instruction
 // and what goes beside it), and where the registers hold it (WAVES) two waves a SIMD fill
 // each other's gaps.
-template <int D, bool FP8, int NW, int WAVES>
+template <int D, bool FP8, int NW, int WAVES, bool PAGED>
 __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a) {
     using T = Tile<D, FP8>;
     constexpr int STAGES = 4;
@@ -934,6 +988,11 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
             whole &= exists[0];
             #pragma unroll
             for (int j = 0; j < kSteps; j++) read_k(rings[1], j);
+            PagedLoads<D, FP8, NW> pages;
+            if constexpr (PAGED) {
+                pages.set();
+                pages.look_up(a, run, u + STAGES, stop);
+            }
             for (int n = (plain - u - 1) / STAGES; n > 0; n--) {
                 #pragma unroll
                 for (int i = 0; i < STAGES; i++, u++) {   // unit u, in stage i
@@ -944,7 +1003,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
                         first_half(sc[i % 2], j);
                         // (LDS answers in order: find() after K's reads, before V's)
                         constexpr int kAt = kSteps / 4;
-                        if (j == kAt) find(u + STAGES, i);
+                        if (!PAGED && j == kAt) find(u + STAGES, i);
                         if (j > kAt && 2 * (j - kAt - 1) < kSteps) {
                             read_v(rings[i], 2 * (j - kAt - 1));
                             read_v(rings[i], 2 * (j - kAt - 1) + 1);
@@ -952,7 +1011,12 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
                         step();
                     }
                     arrive<kIssue>();   // unit u + 2; unit u has been read
-                    issue(i);
+                    if constexpr (PAGED) {
+                        exists[i] = pages.issue(a, o.h, rings[i], rings[i] + my_scales) ? 0xFFFFFFFFu : 0;
+                        pages.look_up(a, run, u + STAGES + 1, stop);
+                    } else {
+                        issue(i);
+                    }
                     #pragma unroll
                     for (int j = 0; j < kSteps; j++) {
                         with_v(j);
@@ -1158,11 +1222,17 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
                 if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2>, nw * kLanes);
             if (!p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, stages, 1>, nw * kLanes);
         }
-        else if (p.kind == kMany) rc = launch(attend_rows_kernel<D, f8, 4, D < 256 ? 2 : 1>, 4 * kLanes);
+        else if (p.kind == kMany) {
+            if constexpr (D == 256)
+                rc = page % 16 == 0 ? launch(attend_rows_kernel<D, f8, 4, 1, true>, 4 * kLanes)
+                                    : launch(attend_rows_kernel<D, f8, 4, 1, false>, 4 * kLanes);
+            else
+                rc = launch(attend_rows_kernel<D, f8, 4, 2, false>, 4 * kLanes);
+        }
         else {
             if constexpr (D < 256) {
                 if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1>, nw * kLanes);
-                else rc = launch(attend_rows_kernel<D, f8, 8, 2>, 8 * kLanes);
+                else rc = launch(attend_rows_kernel<D, f8, 8, 2, false>, 8 * kLanes);
             } else {
                 rc = fail(TANS_EINVAL, "tree_attention: no such kernel");   // (not reached: plan())
             }
