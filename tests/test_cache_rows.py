@@ -55,6 +55,7 @@ extern "C" void plan_(int64_t N, int64_t B, int64_t Hq, int64_t heads, int64_t d
                          p.blocks, p.parts_bytes, p.bytes};
     for (int i = 0; i < 10; i++) o[i] = v[i];
 }
+extern "C" int run_of_(int i, int groups) { return run_of(i, groups); }
 extern "C" int groups_(int least, int groups, int64_t all) {
     Work w = {};
     w.least = least, w.groups = groups;
@@ -151,6 +152,15 @@ def _batches(n, seed):
             16 * int(20000 ** rng.random())
 
 
+@pytest.mark.parametrize("groups", [1, 7, 8, 60, 256, 304, 512, 513])
+def test_every_run_has_its_workgroup(lib, groups):
+    runs = [lib.run_of_(i, groups) for i in range(groups)]
+    assert sorted(runs) == list(range(groups))
+    if groups % 8 == 0:   # an XCD's workgroups have runs that follow each other
+        for x in range(8):
+            assert runs[x::8] == list(range(x * groups // 8, (x + 1) * groups // 8))
+
+
 @pytest.mark.parametrize("cus", [1, 64, 256, 304])
 def test_plans(lib, cus):
     seen = set()
@@ -163,7 +173,9 @@ def test_plans(lib, cus):
             # a workgroup for each item at least, whatever the sequences' tokens
             assert p["blocks"] >= heads * sum(-(-t * G // p["rows"]) for t in counts) and p["bytes"] == 0
         else:
-            assert p["blocks"] == p["groups"] == cus * (2 if p["pairs"] else 1)
+            # two workgroups a CU where the plan says so, and of 128 rows with D below 256
+            two = p["pairs"] or (p["kind"] == MANY and D < 256)
+            assert p["blocks"] == p["groups"] == cus * (2 if two else 1)
             # two parts of a tile and its rows' statistics for each workgroup, and its record
             assert p["parts"] == p["groups"] * 2 * p["rows"] * (D + 2) * 4
             assert p["bytes"] == p["parts"] + p["groups"] * 20
