@@ -57,8 +57,11 @@ constexpr int kXcds = 8;
 TANS_BOTH int run_of(int i, int groups) { return groups % kXcds ? i : i % kXcds * (groups / kXcds) + i / kXcds; }
 
 // Rows of q of a tile: 32 or 64, of which each wave takes all and the waves share the
-// slots, or 128 or 256, of which each wave takes a quarter and the slots pass through
-// LDS once for all.
+// slots, or 128 or 256, of which each of 4 or 8 waves takes 32 and the slots pass through
+// LDS once for all.  256 rows read K and V half as often; below 1024 rows an odd number of
+// 128s is taken as such, where the last tile of 256 would be half empty (a tree of 61
+// tokens, 305 rows, over 32771 slots: 97 us, 102 with tiles of 256; in 8 bits 88 / 111).
+// D = 256 has the registers for 32 rows a wave and one wave a SIMD only.
 enum Kind { kFew, kSome, kMany, kMost };
 struct Plan {
     Kind kind;
