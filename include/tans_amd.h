@@ -438,7 +438,8 @@ int tans_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k
  *   workspace   device scratch of tans_tree_attention_workspace's size (slots
  *               = per * page), 16-byte aligned (contents on entry do not
  *               matter; NULL if 0); calls that overlap in time need one each
- *   out         bf16 [N, q_heads, dim], contiguous, not q
+ *   mask_cols   at least 1 if there is a mask
+ *   out         bf16 [N, q_heads, dim], contiguous; may be q where that is
  * N q_heads below 2^31.                                                  */
 int tans_tree_attention_workspace(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim,
                                   int64_t slots, int64_t max_tokens, int64_t* bytes);

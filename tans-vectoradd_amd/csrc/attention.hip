@@ -1177,8 +1177,8 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
     int rc = batch_check(op, k_cache, v_cache, k_scale, v_scale, pages, heads, page, dim, table, per,
                          starts, lens, B, N, q_heads);
     if (rc != TANS_OK) return rc;
-    if (mask && (mask_cols < 0 || mask_cols > INT32_MAX))
-        return fail(TANS_EINVAL, op + ": the mask must have 0 .. 2^31 - 1 columns");
+    if (mask && (mask_cols < 1 || mask_cols > INT32_MAX))
+        return fail(TANS_EINVAL, op + ": the mask must have 1 .. 2^31 - 1 columns");
     if (!(scale > 0.0f) || scale > 1.0e38f) return fail(TANS_EINVAL, op + ": scale must be positive and finite");
     if (max_tokens < 0) return fail(TANS_EINVAL, op + ": max_tokens must not be negative");
     if (N > INT32_MAX / q_heads) return fail(TANS_EINVAL, op + ": N times the query heads must be below 2^31");

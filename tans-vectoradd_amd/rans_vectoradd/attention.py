@@ -209,8 +209,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     8-bit cache gets each row as fp8_quantize_rows would round it, from 32 bits.
 
     pages int32 [B, pages of a sequence], starts int32 [B + 1], lens int32 [B] (the
-    slots that the cache holds before these tokens).  Every slot must belong to one
-    token: of sequences that share a page, one at most may write to it.  positions are
+    slots that the cache holds before these tokens).  out may be q where q is contiguous.
+    Every slot must belong to one token: of sequences that share a page, one at most may write to it.  positions are
     the tokens' own (in a tree those of its levels), and need not be their slots."""
     N, Hq, D, sq = _heads("q", q)
     dev = q.device
@@ -261,7 +261,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
 
     pages, starts and lens as for rotary_append.  scale (default D ** -0.5) is positive.
     max_tokens: the most new tokens of a sequence (default: the mask's columns, or N);
-    it chooses the kernel, and any value is right.
+    it chooses the kernel, and any value is right.  out may be q where q is contiguous.
 
     Scores, maxima and sums are held in 32 bits; the probabilities are rounded to bf16
     for the product with the values.  A call's result is the same bits every time."""

@@ -93,7 +93,8 @@ def test_attention_refuses():
     for scale in (0.0, -1.0, float("inf"), float("nan"), 2e38):
         assert attend(scale=scale) == -1 and _says(b"scale"), scale
     assert attend(most=-1) == -1 and _says(b"max_tokens")
-    assert attend(mask=D16, cols=-1) == -1 and _says(b"columns")
+    for cols in (-1, 0, 1 << 31):
+        assert attend(mask=D16, cols=cols) == -1 and _says(b"columns"), cols
     assert attend(N=1 << 28) == -1 and _says(b"2^31")
     n = ctypes.c_int64(-1)
 

@@ -224,3 +224,48 @@ def test_buffers_and_masks_of_other_widths():
                        R.tree_attention(*a, two))
     assert (R.tree_attention(*a, torch.ones(4, 0, dtype=torch.bool, device="cuda")) == 0).all()
     assert math.isfinite(whole.float().abs().max().item())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_outputs_over_the_queries(D, fp8):
+    """In every kernel, whole items and shared ones."""
+    import rans_vectoradd as R
+    g = _gen(D)
+    for tokens, context in ((1, 90), (1, 3000), (9, 2000), (13, 500), (30, 1500), (70, 20), (70, 2500)):
+        cache = make_cache(g, -(-(context + tokens) // 16), 4, 16, D, fp8)
+        pages = torch.arange(cache.k.shape[0], dtype=torch.int32).cuda().view(1, -1)
+        q = _randn(g, tokens, 16, D).to(torch.bfloat16)
+        want = R.tree_attention(q, cache, pages, _i32(0, tokens), _i32(context))
+        same = q.clone()
+        assert R.tree_attention(same, cache, pages, _i32(0, tokens), _i32(context), out=same) is same
+        assert torch.equal(same, want), (tokens, context)
+    k, v = (_randn(g, 70, 4, D).to(torch.bfloat16) for _ in range(2))
+    f, _ = R.rotary_frequencies(D)
+    pos = torch.arange(70, dtype=torch.int32).cuda()
+    for interleaved in (False, True):
+        want = R.rotary(q, pos, f, interleaved=interleaved)
+        same = q.clone()
+        R.rotary_append(same, k, v, pos, f, cache, pages, _i32(0, 70), _i32(context), interleaved=interleaved, out=same)
+        assert torch.equal(same, want)
+
+
+def test_many_sequences_of_nothing():
+    """Sequences without new tokens between others, none at all, and B above the tokens."""
+    import rans_vectoradd as R
+    g = _gen(6)
+    cache = make_cache(g, 40, 2, 16, 64, False)
+    B = 1000
+    pages = torch.randint(0, 40, (B, 12), generator=g, device="cuda").to(torch.int32)
+    counts = [1 if b % 97 == 5 else 0 for b in range(B)]
+    starts = _i32(*[sum(counts[:b]) for b in range(B + 1)])
+    lens = torch.randint(0, 150, (B,), generator=g, device="cuda").to(torch.int32)
+    q = _randn(g, sum(counts), 6, 64).to(torch.bfloat16)
+    compare(q, cache, pages, starts, lens, max_tokens=1)
+    out = torch.full_like(q, 4.0)
+    R.tree_attention(q, cache, pages, torch.zeros_like(starts), lens, out=out)
+    assert (out == 4).all()
+    wide = torch.cat((pages, pages), dim=1)   # (items shared by workgroups, none of them any)
+    R.tree_attention(q, cache, wide, torch.zeros_like(starts), lens, out=out)
+    assert (out == 4).all()
+    compare(q, cache, wide, starts, lens, max_tokens=1)
