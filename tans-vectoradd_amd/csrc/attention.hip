@@ -1227,15 +1227,13 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
             if constexpr (few_pairs(D, f8))
                 if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2>, nw * kLanes);
             if (!p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, stages, 1>, nw * kLanes);
-        }
-        else if (p.kind == kMany) {
+        } else if (p.kind == kMany) {
             if constexpr (D == 256)
                 rc = page % 16 == 0 ? launch(attend_rows_kernel<D, f8, 4, 1, true>, 4 * kLanes)
                                     : launch(attend_rows_kernel<D, f8, 4, 1, false>, 4 * kLanes);
             else
                 rc = launch(attend_rows_kernel<D, f8, 4, 2, false>, 4 * kLanes);
-        }
-        else {
+        } else {
             if constexpr (D < 256) {
                 if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1>, nw * kLanes);
                 else rc = launch(attend_rows_kernel<D, f8, 8, 2, false>, 8 * kLanes);

@@ -77,7 +77,9 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
                  int64_t slots, int64_t max_tokens, int cus) {
     const int64_t G = q_heads / heads, rows = max_tokens * G;
     Plan p = {};
-    p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome : rows <= 128 || dim == 256 || ((rows + 127) / 128 % 2 == 1 && rows < 1024) ? kMany : kMost;
+    const bool odd = (rows + 127) / 128 % 2 == 1 && rows < 1024;
+    p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome
+             : rows <= 128 || dim == 256 || odd ? kMany : kMost;
     p.work.rows = 32 << p.kind;
     // no more items than this
     const int64_t items = (N * G / p.work.rows + std::min(N, B)) * heads;
