@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -55,16 +56,20 @@ def build(asm: bool = False) -> str:
     codec_o = os.path.join(BUILD, "codec.o")
     kern_o = os.path.join(BUILD, "kernels.o")
     enc_o = os.path.join(BUILD, "encode.o")
-    _run(["g++", *CXX_FLAGS, "-c", os.path.join(CSRC, "codec.cpp"), "-o", codec_o])
-    _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "-c", os.path.join(CSRC, "kernels.hip"),
-          "-o", kern_o])
-    _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, "encode.hip"), "-o", enc_o])
     layer_o = [os.path.join(BUILD, f"{name}.o") for name in LAYER_SOURCES]
-    for name, obj in zip(LAYER_SOURCES, layer_o):
-        _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj])
+    hip = [HIPCC, *HIP_FLAGS]
+    kernels = [*hip, *KERNEL_FLAGS]
+    steps = [["g++", *CXX_FLAGS, "-c", os.path.join(CSRC, "codec.cpp"), "-o", codec_o],
+             [*kernels, "-c", os.path.join(CSRC, "kernels.hip"), "-o", kern_o],
+             [*hip, "-c", os.path.join(CSRC, "encode.hip"), "-o", enc_o]]
+    steps += [[*hip, "-c", os.path.join(CSRC, f"{name}.hip"), "-o", obj]
+              for name, obj in zip(LAYER_SOURCES, layer_o)]
     if asm:
-        _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "--cuda-device-only", "-S",
-              os.path.join(CSRC, "kernels.hip"), "-o", os.path.join(BUILD, "kernels.s")])
+        steps.append([*kernels, "--cuda-device-only", "-S", os.path.join(CSRC, "kernels.hip"),
+                      "-o", os.path.join(BUILD, "kernels.s")])
+    # (the files one beside the other: a few of them take minutes)
+    with ThreadPoolExecutor(4) as pool:
+        list(pool.map(_run, steps))
     tmp = OUT + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, codec_o, kern_o, enc_o,
           *layer_o, "-lgomp"])
