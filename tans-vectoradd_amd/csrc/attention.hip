@@ -281,7 +281,7 @@ struct Places {
 
 // A tile's 32 rows of q, lane (g, r) holding row r's operands.
 template <int D, bool FP8>
-__device__ __forceinline__ void load_query(const Args& a, const uint16_t* p, bool exists, v8bf (&q)[D / 16]) {
+__device__ __forceinline__ void load_query(const uint16_t* p, bool exists, v8bf (&q)[D / 16]) {
     const int g = (threadIdx.x & (kLanes - 1)) >> 5;
     #pragma unroll
     for (int j = 0; j < D / 16; j++) {
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
             const int row = o.tile * kRows + 32 * t + r;
             mask[t].token = row < rows ? row / a.G : -1;
             mask[t].start = s.start;
-            load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask[t].token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
+            load_query<D, FP8>(a.q + (int64_t)(s.start + mask[t].token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
                                row < rows, q[t]);
             sums[t].clear();
         }
@@ -900,7 +900,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
         Sums<D> sums;
         mask.token = row < rows ? row / a.G : -1;
         mask.start = s.start;
-        load_query<D, FP8>(a, a.q + (int64_t)(s.start + mask.token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
+        load_query<D, FP8>(a.q + (int64_t)(s.start + mask.token) * a.q_stride + (int64_t)(o.h * a.G + row % a.G) * D,
                            row < rows, q);
         sums.clear();
         uint32_t exists[STAGES];
