@@ -59,6 +59,15 @@ struct Batch {
         const int64_t c = lens[b];
         return (int)(c < 0 ? 0 : c < capacity() ? c : capacity());
     }
+    // Whether row n is one of sequence b's tokens, for the b that find_sequence gives: -1
+    // before the first, and where starts go back maybe one that begins behind the row.
+    TANS_BOTH bool owns(int b, int n) const { return b >= 0 && n >= start(b) && n < start(b + 1); }
+    // The slot of row n, which sequence b owns; false if it lies past the table's.
+    TANS_BOTH bool slot_of(int b, int n, uint32_t& s) const {
+        const int64_t i = (int64_t)context(b) + (n - start(b));
+        s = (uint32_t)i;
+        return i < capacity();
+    }
     // Row of the cache (of all heads' and pages') of slot s < capacity() and head h;
     // false if the table's entry is no page.
     TANS_BOTH bool row(int b, uint32_t s, uint32_t h, uint32_t& r) const {

@@ -159,11 +159,11 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows q, Rows k, Rows v
     Share s;
     if (!s.set(waves, r.D / 16, batch.N)) return;   // (whole waves: D / 16 divides 64)
     const int b = find_sequence(batch, s.token);
-    if (b < 0 || s.token >= batch.start(b + 1)) return;
+    if (!batch.owns(b, s.token)) return;
     Chunk<INTER> c;
     c.set(r, s.chunk, s.token);
-    const int64_t slot = (int64_t)batch.context(b) + (s.token - batch.start(b));
-    const bool fits = slot < batch.capacity();
+    uint32_t slot;
+    const bool fits = batch.slot_of(b, s.token, slot);
     const int Hkv = (int)batch.heads, H = Hq + 2 * Hkv;
     auto place = [&](int h) {
         return h < Hq ? q.p + s.token * q.stride + h * r.D
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows q, Rows k, Rows v
             }
             const bool key = h < Hq + Hkv;
             uint32_t row;
-            if (!fits || !batch.row(b, (uint32_t)slot, (uint32_t)(h - Hq - (key ? 0 : Hkv)), row)) continue;
+            if (!fits || !batch.row(b, slot, (uint32_t)(h - Hq - (key ? 0 : Hkv)), row)) continue;
             void* to = key ? cache.k : cache.v;
             if constexpr (FP8) {
                 uint8_t* p = (uint8_t*)to + (int64_t)row * r.D;
