@@ -546,16 +546,11 @@ struct Run {
         }
         return true;
     }
-    // The units of an item that are computed end here: without a mask no row of the tile
-    // sees a slot past its last token's.
     __device__ __forceinline__ int stop(const Args& a, const Item& o, int rows) const {
-        if (a.mask) return o.end;
-        const int last = min(s.tokens - 1, (o.tile * rows + rows - 1) / a.G);
-        return min(o.end, slot_units((int)min((int64_t)s.slots, (int64_t)s.context + last + 1)));
+        return tile_stop(a.mask, s.context, s.tokens, s.slots, o.tile, rows, a.G, o.end);
     }
-    // Below it every row of the tile sees all of a unit's slots, if they exist.
     __device__ __forceinline__ int plain(const Args& a, const Item& o, int rows, int stop) const {
-        return min(stop, (int)(((int64_t)s.context + (a.mask ? 0 : o.tile * rows / a.G + 1)) / kUnit));
+        return tile_plain(a.mask, s.context, s.slots, o.tile, rows, a.G, stop);
     }
 };
 
@@ -633,7 +628,8 @@ struct PagedLoads {
             offset[i] = lane / T::pieces * T::RB + ((lane % T::pieces) ^ key) * 16;
         }
     }
-    // (the table through the scalar cache: nothing writes to it meanwhile)
+    // (the table through the scalar cache: nothing writes to it meanwhile; it has an entry,
+    // since this runs beside plain units, whose slots the sequence has)
     __device__ __forceinline__ void look_up(const Args& a, const Run& run, int u, int stop) {
         const auto* table = (const __attribute__((address_space(4))) int32_t*)a.batch.table + (int64_t)run.b * a.batch.per;
         #pragma unroll

@@ -36,6 +36,21 @@ TANS_BOTH int slot_units(int slots) {
     return slots > 0 ? (int)(((int64_t)slots + kUnit - 1) / kUnit) : 1;
 }
 
+// Of row tile `tile` (rows of G query heads a token, token by token) of a sequence of
+// `tokens` new ones, `context` slots before them and `slots` in all: the units that are
+// computed end at stop, with a mask at `end`, without one behind the slot of the tile's last
+// token; below plain, at most stop, all of a unit's slots are the sequence's and every row of
+// the tile sees them.
+TANS_BOTH int tile_stop(bool masked, int context, int tokens, int slots, int tile, int rows, int G, int end) {
+    if (masked) return end;
+    const int last = std::min(tokens - 1, (tile * rows + rows - 1) / G);
+    return std::min(end, slot_units((int)std::min((int64_t)slots, (int64_t)context + last + 1)));
+}
+TANS_BOTH int tile_plain(bool masked, int context, int slots, int tile, int rows, int G, int stop) {
+    const int64_t seen = (int64_t)context + (masked ? 0 : tile * rows / G + 1);
+    return std::min(stop, (int)(std::min((int64_t)slots, seen) / kUnit));
+}
+
 // Workgroups that share `all` pieces.
 TANS_BOTH int work_groups(const Work& w, int64_t all) {
     const int64_t most = (all + w.least - 1) / w.least;
