@@ -131,9 +131,17 @@ def _heads(name: str, x, dev: Optional[torch.device] = None):
     return N, H, D, a
 
 
+def _factor(name: str, v) -> float:
+    _require(not (isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled()),
+             f"{name} requires a gradient; the attention operators have no backward")
+    return _number(name, v)
+
+
 def _out(out, q, N: int, H: int, D: int):
     if out is None:
         return torch.empty(N, H, D, dtype=_BF16, device=q.device)
+    if _forward._current_level >= 0:   # (it would keep the tangent of what is written over)
+        _no_tangents(out=out)
     if not (_ok(out, _BF16, q.device) and out.shape == (N, H, D)):
         _explain("out", out, _BF16, q.device)
         _require(False, f"out must be {[N, H, D]}")
@@ -157,12 +165,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     N, H, D, stride = _heads("x", x)
     dev = x.device
     if _forward._current_level >= 0:
-        _no_tangents(x=x, positions=positions, frequencies=frequencies)
+        _no_tangents(x=x, frequencies=frequencies, magnitude=magnitude)
     half = frequencies.numel() if isinstance(frequencies, torch.Tensor) else 0
     f = _vector("frequencies", frequencies, _F64, dev, half, "rot / 2")
     p = _vector("positions", positions, _I32, dev, N, "N")
     if type(magnitude) is not float:
-        magnitude = _number("magnitude", magnitude)
+        magnitude = _factor("magnitude", magnitude)
     y = _out(out, x, N, H, D)
     _call(dev, "rotary", lib.tans_rotary, x.data_ptr(), stride, p, f, N, H, D, 2 * half,
           bool(interleaved), bool(inverse), magnitude, y.data_ptr(), H * D)
@@ -175,6 +183,9 @@ def _cache(cache, dev: torch.device):
         k, v, ks, vs = cache
     except (TypeError, ValueError):
         raise RuntimeError("cache must be a KvCache") from None
+    if _forward._current_level >= 0:
+        _no_tangents(**{"the cache's k": k, "the cache's v": v, "the cache's k_scale": ks,
+                        "the cache's v_scale": vs})
     dtype = _BF16 if ks is None and vs is None else _U8
     if not (_ok(k, dtype, dev) and _ok(v, dtype, dev) and k.dim() == 4 and v.shape == k.shape):
         _explain("the cache's k", k, dtype, dev)
@@ -217,7 +228,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     nk, hk, dk, sk = _heads("k", k, dev)
     nv, hv, dv, sv = _heads("v", v, dev)
     if _forward._current_level >= 0:
-        _no_tangents(q=q, k=k, v=v, frequencies=frequencies)
+        _no_tangents(q=q, k=k, v=v, frequencies=frequencies, magnitude=magnitude)
     kc = _cache(cache, dev)
     bt = _batch(pages, starts, lens, dev)
     if not (nk == nv == N and hk == hv == kc[5] and D == dk == dv == kc[7]):
@@ -226,7 +237,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     f = _vector("frequencies", frequencies, _F64, dev, half, "rot / 2")
     p = _vector("positions", positions, _I32, dev, N, "N")
     if type(magnitude) is not float:
-        magnitude = _number("magnitude", magnitude)
+        magnitude = _factor("magnitude", magnitude)
     y = _out(out, q, N, Hq, D)
     _call(dev, "rotary_append", lib.tans_rotary_append, q.data_ptr(), sq, k.data_ptr(), sk,
           v.data_ptr(), sv, p, f, 2 * half, bool(interleaved), magnitude, *kc, *bt, N, Hq,
@@ -268,7 +279,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     N, Hq, D, stride = _heads("q", q)
     dev = q.device
     if _forward._current_level >= 0:
-        _no_tangents(q=q)
+        _no_tangents(q=q, scale=scale)
     kc = _cache(cache, dev)
     bt = _batch(pages, starts, lens, dev)
     if D != kc[7]:
@@ -281,7 +292,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
         if mask.shape[1] == 0:   # (a tensor without elements has no address)
             mask = torch.zeros(N, 1, dtype=torch.bool, device=dev)
         m, W = mask.data_ptr(), mask.shape[1]
-    scale = D ** -0.5 if scale is None else scale if type(scale) is float else _number("scale", scale)
+    scale = D ** -0.5 if scale is None else scale if type(scale) is float else _factor("scale", scale)
     if max_tokens is None:
         most = W or N
     else:
