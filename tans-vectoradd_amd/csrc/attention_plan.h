@@ -90,7 +90,8 @@ constexpr bool few_pairs(int64_t dim, bool eight) { return dim * (eight ? 1 : 2)
 
 inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, bool eight,
                  int64_t slots, int64_t max_tokens, int cus) {
-    const int64_t G = q_heads / heads, rows = max_tokens * G;
+    // (any number of tokens may be given: no sequence has more than INT32_MAX)
+    const int64_t G = q_heads / heads, rows = std::min<int64_t>(max_tokens, INT32_MAX) * G;
     Plan p = {};
     const bool odd = (rows + 127) / 128 % 2 == 1 && rows < 1024;
     p.kind = rows <= 32 ? kFew : rows <= 64 && dim < 256 ? kSome
