@@ -66,7 +66,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
 __device__ __forceinline__ int64_t cost(const Args& a, int b) {
     if (b >= a.batch.B) return 0;
     const Seq s = sequence(a, b);
-    return (int64_t)a.batch.heads * s.tiles * (a.work.whole ? 1 : s.units + a.work.item);
+    return pieces_of(a.work, a.batch.heads, s.tiles, s.units);
 }
 
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -76,11 +76,11 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 
 // The work of all sequences.
 __device__ __forceinline__ int64_t total_cost(const Args& a) {
-    if (a.batch.B == 1) return uniform(cost(a, 0));
+    if (a.batch.B == 1) return uniform(add_pieces(a.work, 0, cost(a, 0)));
     int64_t all = 0;
-    for (int i = threadIdx.x & (kLanes - 1); i < a.batch.B; i += kLanes) all += cost(a, i);
+    for (int i = threadIdx.x & (kLanes - 1); i < a.batch.B; i += kLanes) all = add_pieces(a.work, all, cost(a, i));
     #pragma unroll
-    for (int i = 1; i < kLanes; i *= 2) all += __shfl_xor(all, i);
+    for (int i = 1; i < kLanes; i *= 2) all = add_pieces(a.work, all, __shfl_xor(all, i));
     return uniform(all);
 }
 

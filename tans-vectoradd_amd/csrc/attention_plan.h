@@ -25,7 +25,11 @@ struct Work {
     int least;
     int item;      // pieces that an item counts besides its units
     int whole;
+    // pieces that no batch exceeds, unless its starts go back: sequences that overlap could hold
+    // any number, so they are counted up to here only (what lies behind is not computed)
+    int64_t most;
 };
+constexpr int64_t kMostPieces = int64_t(1) << 50;   // (weeks of work)
 
 TANS_BOTH int row_tiles(int64_t tokens, int64_t G, int rows) {
     return (int)((tokens * G + rows - 1) / rows);
@@ -51,6 +55,12 @@ TANS_BOTH int tile_plain(bool masked, int context, int slots, int tile, int rows
     return std::min(stop, (int)(std::min((int64_t)slots, seen) / kUnit));
 }
 
+// Pieces of a sequence, and of several.
+TANS_BOTH int64_t pieces_of(const Work& w, int64_t heads, int tiles, int units) {
+    return heads * tiles * (w.whole ? 1 : units + w.item);
+}
+TANS_BOTH int64_t add_pieces(const Work& w, int64_t all, int64_t more) { return std::min(all + more, w.most); }
+
 // Workgroups that share `all` pieces.
 TANS_BOTH int work_groups(const Work& w, int64_t all) {
     const int64_t most = (all + w.least - 1) / w.least;
@@ -58,12 +68,12 @@ TANS_BOTH int work_groups(const Work& w, int64_t all) {
 }
 
 // First piece of workgroup i < groups, and the workgroup of piece `at`: the last one
-// that starts at or before it.  (all is below 2^48: 2^30 rows' tiles of 2^26 units over
-// 65535 heads would be more, but not in any memory; groups are below 2^12.)
+// that starts at or before it.  (all is at most kMostPieces, groups are below 2^12; an item
+// that is not counted to its end has pieces from all on, which are the last workgroup's.)
 TANS_BOTH int64_t range_start(int64_t all, int groups, int i) { return all * i / groups; }
 TANS_BOTH int range_of(int64_t all, int groups, int64_t at) {
     // all i / groups <= at, so i < (at + 1) groups / all
-    return (int)(((at + 1) * groups - 1) / all);
+    return at < all ? (int)(((at + 1) * groups - 1) / all) : groups - 1;
 }
 
 // The run of workgroup i of `groups`: workgroups go to the 8 XCDs in turn, and XCD x takes
@@ -108,6 +118,7 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
     p.work.whole = slots <= 8 * kUnit ||
                    (p.kind < kMany && dim < 256 && slots <= 24 * kUnit && items <= 2 * (int64_t)cus) ||
                    (p.kind >= kMany && items >= 4 * (int64_t)cus);
+    p.work.most = std::min(p.work.whole ? items : items * (slot_units((int)slots) + p.work.item), kMostPieces);
     if (p.work.whole) {
         p.blocks = items;
         return p;
