@@ -80,14 +80,21 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", f
     _require(1.0 < base < math.inf and 1.0 <= factor < math.inf, "base must be above 1 and factor at least 1")
     i = torch.arange(dim // 2, dtype=_F64)
     if scaling == "ntk":
-        base *= factor ** (dim / (dim - 2))
+        try:
+            base *= factor ** (dim / (dim - 2))
+        except OverflowError:
+            base = math.inf
+        _require(base < math.inf, "the base, enlarged by the factor, is out of range")
     f = base ** (-2.0 * i / dim)
     magnitude = 1.0
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
         fast, slow = _number("fast", fast), _number("slow", slow)
+        original_length = _number("original_length", original_length)
         _require(fast > slow > 0.0 and original_length >= 1, "yarn needs fast > slow > 0 and an original length")
+        _require(slow > 1e-100 and max(fast, original_length) < 1e100,
+                 "yarn needs fast, slow and an original length within 1e-100 .. 1e100")
 
         def pair(turns):   # the pair that turns so often within the trained length
             return dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
