@@ -39,6 +39,10 @@ __all__ = ["KvCache", "rotary", "rotary_append", "rotary_frequencies", "tree_att
 
 _I32, _F64 = torch.int32, torch.float64
 
+# Marks tensors that a kernel wrote to as changed, for those who saved them for a backward
+# pass: 0.2 us, and 0.9 through the public function's own checks.
+_changed = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
 
 class KvCache(NamedTuple):
     """k, v: bf16 [pages, heads, page, D], or uint8 (E4M3FN bytes) with a float32
@@ -181,6 +185,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     y = _out(out, x, N, H, D)
     _call(dev, "rotary", lib.tans_rotary, x.data_ptr(), stride, p, f, N, H, D, 2 * half,
           bool(interleaved), bool(inverse), magnitude, y.data_ptr(), H * D)
+    if out is not None:
+        _changed((out,))
     return y
 
 
@@ -249,6 +255,9 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     _call(dev, "rotary_append", lib.tans_rotary_append, q.data_ptr(), sq, k.data_ptr(), sk,
           v.data_ptr(), sv, p, f, 2 * half, bool(interleaved), magnitude, *kc, *bt, N, Hq,
           y.data_ptr())
+    _changed(cache[:2] if kc[2] is None else cache)
+    if out is not None:
+        _changed((out,))
     return y
 
 
@@ -310,4 +319,6 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     ws = torch.empty(need, dtype=_U8, device=dev) if need else None
     _call(dev, "tree_attention", lib.tans_tree_attention, q.data_ptr(), stride, *kc, *bt, m, W, N, Hq,
           scale, most, None if ws is None else ws.data_ptr(), need, y.data_ptr())
+    if out is not None:
+        _changed((out,))
     return y
