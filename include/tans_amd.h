@@ -431,7 +431,9 @@ int tans_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k
  * columns it lacks are 0), or without a mask (NULL) i <= t for token t of its
  * sequence.  A token that sees nothing gets zeros, and what it does not see
  * does not reach it.  Scores and sums in fp32, probabilities rounded to bf16
- * for the product with v; a fixed order, without atomics.
+ * for the product with v (8-bit rows: after v's scales), or held in 16 bits
+ * where a bf16 cache's items of few rows are shared by workgroups; a fixed
+ * order, without atomics.
  *   scale       positive, finite
  *   max_tokens  about the most new tokens of a sequence: chooses the kernel,
  *               any value >= 0 is right (the same for both calls)

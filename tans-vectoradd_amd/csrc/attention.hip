@@ -186,6 +186,13 @@ __device__ __forceinline__ v8bf from_fp8(uint32_t lo, uint32_t hi) {
     return __builtin_bit_cast(v8bf, u);
 }
 
+// Two probabilities as bf16, and what a bf16 cut off leaves of one: 2^-15 of it is lost by
+// both together.  (Never zero of what is not, since an infinite value times it would be NaN.)
+__device__ __forceinline__ uint32_t bf16_cut(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+__device__ __forceinline__ float rest_of(float x, float cut) { return fmaxf(x - cut, x * 7.6293945e-6f); }   // 2^-17
+
 // Infinities and NaN among the values of a 32-bit word: join() gathers words, any() says
 // whether one of them held any, drop() puts zero in their place.
 template <bool FP8> struct Odd;
@@ -348,13 +355,22 @@ __device__ __forceinline__ void read_scales(Lds from, float (&f)[16]) {
 // maximum and sum are one lane's and its other half's.  Those 16 are, rounded to bf16,
 // the operand of O^T = V^T P^T as they lie there, if the slots are taken in that order;
 // V's operand, 8 slots of one dimension, comes from LDS by transposing reads.
+//
+// Rounded to bf16, a probability loses 2^-8 of itself at most, and the result's error against
+// 64 bits becomes 1.2 to 1.5 times that of its own rounding.  It is the type in which the matrix
+// cores multiply by bf16 values without a loss of theirs.  SPLIT holds 16 bits, as the
+// sum of two bf16 that are each multiplied: for shared items of 32 rows of a bf16 cache, whose
+// products wait for memory (one token of 262144 slots 192.0 -> 192.6 us, 7 of 4000 33.1 / 33.1, 256 of
+// 512 128.3 -> 131.6).  Elsewhere it costs too much: one token of 700 slots 12.7 -> 13.9, 8 bits
+// 262144 slots 110 -> 114, 17 trees 39.7 -> 44.6, a tree of 8 with 64 rows 47 -> 51; and tiles of
+// 128 or 256 rows are bound by their products.
 struct Mask {
     int token;         // the lane's row's, in its sequence, or -1
     int start;         // the sequence's first row of q
     int before;        // slots of the context from the unit's first on, 32 at most
     uint32_t exists;   // of the unit's slots
 };
-template <int D, bool FP8, bool MASKED>
+template <int D, bool FP8, bool MASKED, bool SPLIT>
 __device__ __forceinline__ void attend_unit(const Args& a, const Places<D, FP8>& at, Lds stage, Lds scales,
                                             const v8bf (&q)[D / 16], Sums<D>& sums,
                                             const Mask& mask) {
@@ -410,7 +426,7 @@ __device__ __forceinline__ void attend_unit(const Args& a, const Places<D, FP8>&
             if (!(mine >> (i / 4 * 8 + i % 4) & 1)) sc[i] = kNone;
     }
     const float mc = sums.admit(sc, a.c);
-    v8bf p[2];
+    v8bf p[2], rest[2];
     float e[16];
     #pragma unroll
     for (int i = 0; i < 16; i++) {
@@ -420,9 +436,17 @@ __device__ __forceinline__ void attend_unit(const Args& a, const Places<D, FP8>&
         if constexpr (FP8) e[i] = MASKED && e[i] == 0.0f ? 0.0f : e[i] * vs[i];
     }
     #pragma unroll
-    for (int k = 0; k < 2; k++)
-        p[k] = __builtin_bit_cast(v8bf, v4u{bf16_pack(e[8 * k], e[8 * k + 1]), bf16_pack(e[8 * k + 2], e[8 * k + 3]),
-                                            bf16_pack(e[8 * k + 4], e[8 * k + 5]), bf16_pack(e[8 * k + 6], e[8 * k + 7])});
+    for (int k = 0; k < 2; k++) {
+        v4u high, low = {0, 0, 0, 0};
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = e[8 * k + 2 * i], y = e[8 * k + 2 * i + 1];
+            high[i] = SPLIT ? bf16_cut(x, y) : bf16_pack(x, y);
+            if constexpr (SPLIT) low[i] = bf16_pack(rest_of(x, bf16_lo(high[i])), rest_of(y, bf16_hi(high[i])));
+        }
+        p[k] = __builtin_bit_cast(v8bf, high);
+        rest[k] = __builtin_bit_cast(v8bf, low);
+    }
     // A value that is infinite or NaN reaches the rows that see its slot, and by the
     // matrix product it would reach the others as well (0 times it is NaN): it is left out
     // there, and added below.
@@ -448,8 +472,11 @@ __device__ __forceinline__ void attend_unit(const Args& a, const Places<D, FP8>&
     #pragma unroll
     for (int n = 0; n < D / 32; n++)
         #pragma unroll
-        for (int k = 0; k < 2; k++)
-            sums.acc[n] = mfma(FP8 ? from_fp8(vr[n][k][0], vr[n][k][1]) : __builtin_bit_cast(v8bf, vr[n][k]), p[k], sums.acc[n]);
+        for (int k = 0; k < 2; k++) {
+            const v8bf v = FP8 ? from_fp8(vr[n][k][0], vr[n][k][1]) : __builtin_bit_cast(v8bf, vr[n][k]);
+            sums.acc[n] = mfma(v, p[k], sums.acc[n]);
+            if constexpr (SPLIT) sums.acc[n] = mfma(v, rest[k], sums.acc[n]);
+        }
     if constexpr (MASKED) {
         if (odd) {
             for (uint32_t key = 0; key < kUnit; key++) {
@@ -685,7 +712,7 @@ __device__ __forceinline__ int64_t out_row(const Args& a, const Run& run, const 
 // ring's loads under way.  Memory bounds it: one token of 262144 slots, 8 heads, D = 128,
 // 192 us (1.07 GB at 5.6 TB/s); 96 tokens over 100 .. 16000 slots in 8 bits 138 us (648 MB at
 // 4.7 TB/s); D = 256 reaches 4.1-4.4 TB/s, with two waves' rings of 32 KB a unit.
-template <int D, bool FP8, int RT, int NW, int STAGES, int WAVES>
+template <int D, bool FP8, int RT, int NW, int STAGES, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
     using T = Tile<D, FP8>;
     constexpr int kRows = 32 * RT;
@@ -726,7 +753,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
             for (int t = 0; t < RT; t++) {
                 mask[t].before = min(s.context - u * kUnit, kUnit);
                 mask[t].exists = exists;
-                attend_unit<D, FP8, decltype(MASKED)::value>(a, at, stage + mine, stage + mine + 2 * T::bytes, q[t], sums[t], mask[t]);
+                attend_unit<D, FP8, decltype(MASKED)::value, SPLIT>(a, at, stage + mine, stage + mine + 2 * T::bytes, q[t], sums[t], mask[t]);
                 // (the second tile reads the stage again: its operands in registers from one
                 // tile to the next would be more than there are)
                 __builtin_amdgcn_sched_barrier(0);
@@ -1056,7 +1083,7 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_rows_kernel(Args a)
                 mask.exists = exists[0];
                 #pragma unroll
                 for (int k = 1; k < STAGES; k++) mask.exists = i == k ? exists[k] : mask.exists;
-                attend_unit<D, FP8, true>(a, at, stage, stage + my_scales, q, sums, mask);
+                attend_unit<D, FP8, true, false>(a, at, stage, stage + my_scales, q, sums, mask);
             }
             arrive<0>();   // (before the ring is filled again)
             if (u < stop) {
@@ -1221,8 +1248,10 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
         if (p.kind == kFew) {
             rc = TANS_EINVAL;
             if constexpr (few_pairs(D, f8))
-                if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2>, nw * kLanes);
-            if (!p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, stages, 1>, nw * kLanes);
+                if (p.pairs) rc = launch(attend_kernel<D, f8, 1, nw, pair_stages, 2, !f8>, nw * kLanes);
+            if (!p.pairs)
+                rc = p.work.whole ? launch(attend_kernel<D, f8, 1, nw, stages, 1, false>, nw * kLanes)
+                                  : launch(attend_kernel<D, f8, 1, nw, stages, 1, !f8>, nw * kLanes);
         } else if (p.kind == kMany) {
             if constexpr (D == 256)
                 rc = page % 16 == 0 ? launch(attend_rows_kernel<D, f8, 4, 1, true>, 4 * kLanes)
@@ -1231,7 +1260,7 @@ int tans_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
                 rc = launch(attend_rows_kernel<D, f8, 4, 2, false>, 4 * kLanes);
         } else {
             if constexpr (D < 256) {
-                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1>, nw * kLanes);
+                if (p.kind == kSome) rc = launch(attend_kernel<D, f8, 2, nw, stages, 1, false>, nw * kLanes);
                 else rc = launch(attend_rows_kernel<D, f8, 8, 2, false>, 8 * kLanes);
             } else {
                 rc = fail(TANS_EINVAL, "tree_attention: no such kernel");   // (not reached: plan())

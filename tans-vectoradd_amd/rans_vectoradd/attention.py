@@ -291,7 +291,10 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     it chooses the kernel, and any value is right.  out may be q where q is contiguous.
 
     Scores, maxima and sums are held in 32 bits; the probabilities are rounded to bf16
-    for the product with the values.  A call's result is the same bits every time."""
+    for the product with the values (of 8-bit rows after the values' scales), or held in
+    16 bits: of a bf16 cache where a sequence's new tokens, times the query heads of a
+    cache head, are 32 rows at most and their slots are shared by workgroups.  A call's
+    result is the same bits every time."""
     N, Hq, D, stride = _heads("q", q)
     dev = q.device
     if _forward._current_level >= 0:
