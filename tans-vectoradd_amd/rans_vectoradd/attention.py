@@ -170,7 +170,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     D at most 1024.
 
     x's tokens may be parts of longer rows (a multiple of 8 elements apart), its start
-    16-byte aligned; out [N, H, D] is contiguous, and may be x itself where x is.
+    16-byte aligned; out [N, H, D] is contiguous, and may be x itself where x is (else
+    they must not overlap).
     inverse: by the negative angle.  Angles are exact to the frequencies' last bit at
     any position; one rounding, to bf16."""
     N, H, D, stride = _heads("x", x)
@@ -191,7 +192,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
 
 
 def _cache(cache, dev: torch.device):
-    """(k, v, scales' addresses, pages, heads, page, D) of a cache."""
+    """((k, v, scales' addresses, pages, heads, page, D), its tensors) of a cache."""
     try:
         k, v, ks, vs = cache
     except (TypeError, ValueError):
@@ -209,8 +210,9 @@ def _cache(cache, dev: torch.device):
         _explain("the cache's k_scale", ks, _F32, dev)
         _explain("the cache's v_scale", vs, _F32, dev)
         _require(False, "the cache's scales must be [pages, heads, page]")
-    return (k.data_ptr(), v.data_ptr(), None if ks is None else ks.data_ptr(),
-            None if vs is None else vs.data_ptr(), pages, heads, page, D)
+    if ks is None:
+        return (k.data_ptr(), v.data_ptr(), None, None, pages, heads, page, D), (k, v)
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, page, D), (k, v, ks, vs)
 
 
 def _batch(pages, starts, lens, dev: torch.device):
@@ -233,16 +235,17 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     8-bit cache gets each row as fp8_quantize_rows would round it, from 32 bits.
 
     pages int32 [B, pages of a sequence], starts int32 [B + 1], lens int32 [B] (the
-    slots that the cache holds before these tokens).  out may be q where q is contiguous.
-    Every slot must belong to one token: of sequences that share a page, one at most may write to it.  positions are
-    the tokens' own (in a tree those of its levels), and need not be their slots."""
+    slots that the cache holds before these tokens).  out may be q where q is contiguous,
+    and must overlap nothing else.  Every slot must belong to one token: of sequences that
+    share a page, one at most may write to it.  positions are the tokens' own (in a tree
+    those of its levels), and need not be their slots."""
     N, Hq, D, sq = _heads("q", q)
     dev = q.device
     nk, hk, dk, sk = _heads("k", k, dev)
     nv, hv, dv, sv = _heads("v", v, dev)
     if _forward._current_level >= 0:
         _no_tangents(q=q, k=k, v=v, frequencies=frequencies, magnitude=magnitude)
-    kc = _cache(cache, dev)
+    kc, held = _cache(cache, dev)
     bt = _batch(pages, starts, lens, dev)
     if not (nk == nv == N and hk == hv == kc[5] and D == dk == dv == kc[7]):
         _require(False, f"q, k, v must be [N, Hq, {kc[7]}] and [N, {kc[5]}, {kc[7]}] as the cache's rows")
@@ -255,7 +258,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     _call(dev, "rotary_append", lib.tans_rotary_append, q.data_ptr(), sq, k.data_ptr(), sk,
           v.data_ptr(), sv, p, f, 2 * half, bool(interleaved), magnitude, *kc, *bt, N, Hq,
           y.data_ptr())
-    _changed(cache[:2] if kc[2] is None else cache)
+    _changed(held)
     if out is not None:
         _changed((out,))
     return y
@@ -289,7 +292,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     pages, starts and lens as for rotary_append.  scale (default D ** -0.5) is positive.
     max_tokens: the most new tokens of a sequence (default: the mask's columns, or the
     tokens of a sequence on average); it chooses the kernel, and any value is right.  out
-    may be q where q is contiguous.
+    may be q where q is contiguous, and must overlap nothing else.
 
     Scores, maxima and sums are held in 32 bits; the probabilities are rounded to bf16
     for the product with the values (of 8-bit rows after the values' scales), or held in
@@ -300,7 +303,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     dev = q.device
     if _forward._current_level >= 0:
         _no_tangents(q=q, scale=scale)
-    kc = _cache(cache, dev)
+    kc, _ = _cache(cache, dev)
     bt = _batch(pages, starts, lens, dev)
     if D != kc[7]:
         _require(False, f"q must be [N, Hq, {kc[7]}] as the cache's rows")
@@ -315,7 +318,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, pages: torch.Tensor, starts:
     scale = D ** -0.5 if scale is None else scale if type(scale) is float else _factor("scale", scale)
     if max_tokens is None:
         # N would be a long prompt's kernel for a batch of single tokens (96 of them over 100 ..
-        # 16000 slots 338 us, so 225, in 8 bits 379 / 138; 255 beside a prompt of 512 639 / 429);
+        # 16000 slots 338 us, so 225, in 8 bits 379 / 138; 255 beside a prompt of 512 647 / 429);
         # worse is the average where one prompt has nearly all of the work (255 over 100 slots
         # beside 2048 tokens over 14000 979 / 1246)
         most = W or -(-N // max(bt[4], 1))
