@@ -357,13 +357,13 @@ __device__ __forceinline__ void read_scales(Lds from, float (&f)[16]) {
 // V's operand, 8 slots of one dimension, comes from LDS by transposing reads.
 //
 // Rounded to bf16, a probability loses 2^-8 of itself at most, and the result's error against
-// 64 bits becomes 1.2 to 1.5 times that of its own rounding.  It is the type in which the matrix
-// cores multiply by bf16 values without a loss of theirs.  SPLIT holds 16 bits, as the
-// sum of two bf16 that are each multiplied: for shared items of 32 rows of a bf16 cache, whose
-// products wait for memory (one token of 262144 slots 192.0 -> 192.6 us, 7 of 4000 33.1 / 33.1, 256 of
-// 512 128.3 -> 131.6).  Elsewhere it costs too much: one token of 700 slots 12.7 -> 13.9, 8 bits
-// 262144 slots 110 -> 114, 17 trees 39.7 -> 44.6, a tree of 8 with 64 rows 47 -> 51; and tiles of
-// 128 or 256 rows are bound by their products.
+// 64 bits becomes about 1.4 times that of its own rounding (1.0 to 1.6 for single rows).  It is
+// the type in which the matrix cores multiply by bf16 values without a loss of theirs.  SPLIT
+// holds 16 bits, as the sum of two bf16 that are each multiplied: for shared items of 32 rows of
+// a bf16 cache, whose products wait for memory (one token of 262144 slots 192.0 -> 192.6 us, 7 of
+// 4000 33.1 / 33.1, 256 of 512 128.3 -> 131.4).  Elsewhere it costs too much: one token of 700
+// slots 12.7 -> 13.9, 8 bits 262144 slots 110 -> 114, 17 trees 39.7 -> 44.6, a tree of 8 with 64
+// rows 47 -> 51; and tiles of 128 or 256 rows are bound by their products.
 struct Mask {
     int token;         // the lane's row's, in its sequence, or -1
     int start;         // the sequence's first row of q
@@ -710,8 +710,10 @@ __device__ __forceinline__ int64_t out_row(const Args& a, const Run& run, const 
 // ring of its own in LDS that loads write without a register between; the waves' sums are
 // added at the end.  Nothing makes the waves wait for each other, so that each keeps its
 // ring's loads under way.  Memory bounds it: one token of 262144 slots, 8 heads, D = 128,
-// 192 us (1.07 GB at 5.6 TB/s); 96 tokens over 100 .. 16000 slots in 8 bits 138 us (648 MB at
-// 4.7 TB/s); D = 256 reaches 4.1-4.4 TB/s, with two waves' rings of 32 KB a unit.
+// 193 us (1.07 GB at 5.6 TB/s); 96 tokens over 100 .. 16000 slots in 8 bits 138 us (648 MB at
+// 4.7 TB/s); D = 256 reaches 4.1-4.4 TB/s, with two waves' rings of 32 KB a unit.  (Some spill
+// registers, up to 45 with D = 256: stored and loaded again at an item's begin and end, not in
+// the loops over its units.)
 template <int D, bool FP8, int RT, int NW, int STAGES, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
     using T = Tile<D, FP8>;
@@ -888,8 +890,8 @@ __global__ __launch_bounds__(NW * kLanes, WAVES) void attend_kernel(Args a) {
 // LDS once for all of them.  A unit's products with K run beside the exponentials of the
 // one before in the same wave's instructions, step by step (a step is a matrix instruction
 // and what goes beside it), and where the registers hold it (WAVES) two waves a SIMD fill
-// each other's gaps.  2048 tokens of 40 heads over 14000 slots and themselves, D = 128: 679 us,
-// 925 TFLOP/s (D = 64 440 us, D = 256 with 16 heads 595, 8 bits 770).  The matrix cores are busy
+// each other's gaps.  2048 tokens of 40 heads over 14000 slots and themselves, D = 128: 672 us,
+// 938 TFLOP/s (D = 64 440 us, D = 256 with 16 heads 605, 8 bits 758).  The matrix cores are busy
 // 43% of the cycles; a quarter of the waves' time is waits (the unit's barrier and LDS), a
 // third waits for its turn to issue.  Two tiles of 32 rows a wave and one wave a SIMD, which
 // reads LDS half as often, took 893 us.

@@ -112,9 +112,10 @@ inline Plan plan(int64_t N, int64_t B, int64_t q_heads, int64_t heads, int64_t d
     p.work.least = 8;
     p.work.item = p.kind >= kMany ? 8 : (int)(196608 / (2 * kUnit * dim * (eight ? 1 : 2)));
     // An item a workgroup, without a second kernel that joins parts: few slots, up to 24 units
-    // where the items are few as well (one token of 700 slots 12.5 us, shared 14.8; 32 sequences of
-    // 512 18.7 / 20.9; but 256 of them 158 / 128, and D = 256, 700 slots 27.9 / 22.3), or so many
-    // items that they fill the CUs evenly.
+    // where the items are few as well (one token of 760 slots 12.8 us, shared 15.3; of 800 13.8 / 15.3,
+    // 1024 15.8 / 15.3; 32 sequences of 512 18.7 / 20.9; but 256 of them 158 / 131, and D = 256, 700
+    // slots 27.9 / 22.3), or so many items that they fill the CUs evenly.  (slots are the table's:
+    // the host does not know the sequences', and a wider table takes the shared path.)
     p.work.whole = slots <= 8 * kUnit ||
                    (p.kind < kMany && dim < 256 && slots <= 24 * kUnit && items <= 2 * (int64_t)cus) ||
                    (p.kind >= kMany && items >= 4 * (int64_t)cus);
